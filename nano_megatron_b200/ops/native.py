@@ -98,6 +98,9 @@ def lib() -> ctypes.CDLL:
                         "(the CUDA ops do not fall back to PyTorch on a GPU)"
                     )
                 _lib = ctypes.CDLL(str(_LIB_PATH))
+                for fn in (_lib.nmb_band_fwd, _lib.nmb_band_bwd):
+                    fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]   # packed arguments, stream
+                _lib.nmb_band_dtable_part.restype = ctypes.c_longlong
                 pair = os.environ.get("NMB_GEMM_PAIR")
                 if pair is not None:
                     _lib.nmb_gemm_set_pair(int(pair != "0"))
@@ -145,7 +148,7 @@ def check_status(device: torch.device | None = None, *, reset: bool = True) -> N
 
 
 #: kernels launched by each C entry point (for launch accounting)
-_KERNELS_PER_CALL = {"nmb_attn_bwd": 3, "nmb_col_reduce": 2, "nmb_adamw_step": 2}
+_KERNELS_PER_CALL = {"nmb_attn_bwd": 3, "nmb_band_bwd": 2, "nmb_col_reduce": 2, "nmb_adamw_step": 2}
 #: running count of kernels of this library launched (or captured) by this process
 launches = 0
 #: the same per C entry point (tests use it to show that a fused path left no stand-alone kernel behind)

@@ -1,0 +1,289 @@
+"""The banded attention kernels against the definition in 64 bits."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests._band_oracle import check, oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _tensors(b, sq, skv, hq, hkv, d, buckets=0, layout="bshd", seed=0, table_dtype=torch.bfloat16, gain=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+    if layout == "packed":
+        assert sq == skv
+        q, k, v = normal(b, sq, (hq + 2 * hkv) * d).split([hq * d, hkv * d, hkv * d], dim=-1)
+        q, k, v = q.unflatten(-1, (hq, d)), k.unflatten(-1, (hkv, d)), v.unflatten(-1, (hkv, d))
+    elif layout == "bhsd":
+        q, k, v = (normal(b, h, s, d).transpose(1, 2) for h, s in ((hq, sq), (hkv, skv), (hkv, skv)))
+    elif layout == "odd":  # rows that tile loads cannot address: the last dimension with a stride, an unaligned start
+        q = normal(b, sq, hq, 2 * d)[..., ::2]
+        k = normal(b * skv * hkv * d + 1)[1:].view(b, skv, hkv, d)
+        v = normal(b, skv, hkv, d + 4)[..., :d]
+    else:
+        q, k, v = normal(b, sq, hq, d), normal(b, skv, hkv, d), normal(b, skv, hkv, d)
+    if gain != 1.0:
+        q = (q.float() * gain).to(torch.bfloat16)
+    table = None
+    if buckets:
+        table = torch.randn(hq, buckets, generator=g, device="cuda").to(table_dtype).requires_grad_(True)
+    return [t.detach().requires_grad_(True) for t in (q, k, v)] + [table, normal(b, sq, hq, d)]
+
+
+def _call(q, k, v, table, scale, max_distance, **kw):
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention, window_attention
+
+    if table is None:
+        return window_attention(q, k, v, scale, **kw)
+    return relative_bias_attention(q, k, v, table, scale, max_distance=max_distance, **kw)
+
+
+def _compare(q, k, v, table, dout, *, window=None, sinks=0, start=0, max_distance=128, scale=None, what=""):
+    from nano_megatron_b200.ops import native
+
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    before = native.launch_counts.get("nmb_band_bwd", 0)
+    out = _call(q, k, v, table, scale, max_distance, window=window, sinks=sinks, query_start=start)
+    leaves = [q, k, v] + ([] if table is None else [table])
+    grads = torch.autograd.grad(out, leaves, dout)
+    torch.cuda.synchronize()
+    native.check_status()
+    assert native.launch_counts["nmb_band_bwd"] == before + 1  # the kernels ran
+    values, bounds, rms = oracle(q, k, v, dout, scale, window=window, sinks=sinks, start=start, table=table, max_distance=max_distance)
+    check(dict(zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads))), values, bounds, rms, what)
+
+
+# b, sq, skv, hq, hkv, d, window, sinks, start
+WINDOWS = [
+    (1, 1, 1, 1, 1, 64, 1, 0, 0), (2, 2, 2, 2, 1, 128, 2, 0, 0), (1, 5, 5, 2, 2, 96, 3, 1, 0),
+    (1, 64, 64, 2, 2, 64, 16, 0, 0), (1, 127, 127, 2, 1, 96, 40, 3, 0), (2, 128, 128, 1, 1, 128, 128, 0, 0),
+    (1, 129, 129, 4, 2, 64, 2, 0, 0), (1, 255, 255, 3, 1, 128, 64, 65, 0), (2, 256, 256, 2, 2, 64, 127, 1, 0),
+    (1, 257, 257, 2, 2, 96, 128, 0, 0), (1, 300, 300, 8, 1, 64, 129, 4, 0), (2, 513, 513, 4, 4, 64, 1, 0, 0),
+    (1, 640, 640, 2, 1, 128, 256, 130, 0), (1, 777, 777, 3, 3, 96, 300, 0, 0), (1, 1000, 1000, 2, 2, 64, 100, 1000, 0),
+    (1, 1100, 1100, 1, 1, 128, 2000, 0, 0),
+    # shards: one row, rows that start inside a tile, few rows over many keys, more keys than rows can see
+    (2, 1, 700, 4, 2, 64, 200, 3, 699), (1, 33, 500, 2, 1, 128, 90, 0, 467), (1, 300, 900, 4, 4, 96, 1000, 0, 600),
+    (1, 200, 900, 2, 2, 64, 64, 5, 100), (1, 130, 2000, 2, 1, 64, 1500, 0, 1870),
+    # shards behind the keys: rows whose window holds no key, with sinks and without
+    (1, 200, 100, 2, 2, 64, 30, 0, 50), (1, 200, 100, 2, 1, 128, 30, 2, 50), (2, 10, 5, 1, 1, 96, 3, 0, 200), (1, 400, 128, 2, 2, 64, 100, 0, 0),
+]
+
+
+@pytest.mark.parametrize("b,sq,skv,hq,hkv,d,window,sinks,start", WINDOWS)
+def test_window(b, sq, skv, hq, hkv, d, window, sinks, start):
+    _compare(*_tensors(b, sq, skv, hq, hkv, d), window=window, sinks=sinks, start=start)
+
+
+# b, sq, skv, hq, hkv, d, window, sinks, start, buckets, max_distance
+BIASES = [
+    (1, 1, 1, 1, 1, 64, None, 0, 0, 2, 2), (2, 3, 3, 2, 1, 128, None, 0, 0, 32, 128), (1, 33, 33, 4, 4, 64, None, 0, 0, 32, 128),
+    (1, 128, 128, 2, 2, 96, None, 0, 0, 32, 128), (2, 200, 200, 4, 2, 64, None, 0, 0, 20, 40), (1, 257, 257, 2, 2, 128, None, 0, 0, 5, 300),
+    (3, 390, 390, 3, 1, 96, None, 0, 0, 128, 256), (1, 700, 700, 2, 2, 64, None, 0, 0, 64, 600), (1, 1300, 1300, 2, 1, 128, None, 0, 0, 32, 128),
+    (1, 600, 600, 2, 2, 64, None, 0, 0, 3, 2), (1, 600, 600, 1, 1, 128, None, 0, 0, 128, 2048),
+    (1, 513, 513, 4, 1, 64, 100, 3, 0, 16, 64), (2, 300, 300, 2, 2, 128, 33, 0, 0, 32, 128), (1, 450, 450, 8, 2, 96, 200, 140, 0, 32, 100),
+    (1, 1, 600, 2, 2, 64, None, 0, 599, 32, 128), (2, 70, 500, 4, 2, 128, None, 0, 430, 32, 128), (1, 150, 700, 2, 1, 96, 120, 4, 333, 32, 128),
+    (1, 200, 90, 2, 2, 64, 40, 0, 60, 16, 30), (1, 200, 90, 2, 2, 64, None, 0, 60, 16, 30),
+]
+
+
+@pytest.mark.parametrize("b,sq,skv,hq,hkv,d,window,sinks,start,buckets,distance", BIASES)
+def test_bias(b, sq, skv, hq, hkv, d, window, sinks, start, buckets, distance):
+    _compare(*_tensors(b, sq, skv, hq, hkv, d, buckets), window=window, sinks=sinks, start=start, max_distance=distance)
+
+
+@pytest.mark.parametrize("layout", ["packed", "bhsd", "odd"])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_layouts(layout, d):
+    _compare(*_tensors(2, 200, 200, 4, 2, d, layout=layout), window=70, sinks=2)
+    _compare(*_tensors(2, 200, 200, 4, 2, d, 32, layout=layout))
+
+
+def test_fp32_table():
+    _compare(*_tensors(2, 300, 300, 4, 2, 64, 32, table_dtype=torch.float32))
+
+
+def test_peaked_scores():
+    # maxima that move by more than the threshold between tiles, in both directions
+    _compare(*_tensors(1, 600, 600, 2, 2, 64, gain=12.0), window=400, sinks=4)
+    _compare(*_tensors(1, 600, 600, 2, 2, 128, 32, gain=12.0))
+
+
+@pytest.mark.parametrize("mask", [-math.inf, torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max])
+@pytest.mark.parametrize("window", [None, 40])
+def test_masked_buckets(mask, window):
+    q, k, v, table, dout = _tensors(1, 400, 400, 4, 2, 64, 16)
+    with torch.no_grad():
+        table[0, 0] = mask      # a head that does not see its own position: its first row sees nothing, or itself after all
+        table[1, 15] = mask     # nothing from some distance on
+        table[2, 3:9] = mask
+        table[3] = mask if mask == -math.inf else table[3]  # a head that sees nothing at all
+    _compare(q, k, v, table, dout, window=window, max_distance=100)
+
+
+def test_rows_of_one_lowest_value_are_averaged():
+    q, k, v, table, dout = _tensors(1, 300, 300, 2, 2, 64, 16)
+    with torch.no_grad():
+        table.fill_(torch.finfo(torch.bfloat16).min)
+        q.zero_()               # the scores add nothing: an even average of the visible keys
+    _compare(q, k, v, table, dout, window=50, max_distance=100)
+
+
+def test_broadcast_inputs_and_gradients():
+    from nano_megatron_b200.ops.band_attention import window_attention
+
+    q, k, v, _, _ = _tensors(1, 150, 150, 4, 1, 64)
+    kb, vb = (t.expand(2, 150, 2, 64) for t in (k, v))
+    qb = q.expand(2, 150, 4, 64)
+    out = window_attention(qb, kb, vb, 0.125, window=40)
+    ones = torch.ones((), device="cuda", dtype=torch.bfloat16).expand(out.shape)
+    grads = torch.autograd.grad(out, (qb, kb, vb), ones, retain_graph=True)
+    values, bounds, rms = oracle(qb, kb, vb, ones, 0.125, window=40)
+    check(dict(zip(("out", "dq", "dk", "dv"), (out, *grads))), values, bounds, rms)
+    out.sum().backward()
+    assert q.grad.shape == q.shape and k.grad.shape == k.shape
+
+
+def test_same_results_twice_and_only_what_is_asked_for():
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention
+
+    q, k, v, table, dout = _tensors(2, 500, 500, 4, 2, 64, 32)
+    runs = []
+    for _ in range(3):
+        out = relative_bias_attention(q, k, v, table, 0.125, window=300, sinks=4)
+        runs.append((out, *torch.autograd.grad(out, (q, k, v, table), dout)))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+    frozen = table.detach()
+    out = relative_bias_attention(q, k, v, frozen, 0.125, window=300, sinks=4)
+    for a, b in zip(runs[0][1:], torch.autograd.grad(out, (q, k, v), dout)):
+        assert torch.equal(a, b)
+
+
+def test_main_grad_of_the_table():
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention
+
+    q, k, v, table, dout = _tensors(1, 200, 200, 2, 2, 64, 16, table_dtype=torch.float32)
+    want = torch.autograd.grad(relative_bias_attention(q, k, v, table, 0.125, max_distance=60), table, dout)[0]
+    param = torch.nn.Parameter(table.detach().clone())
+    for buffer in (torch.ones(2, 16, device="cuda"), torch.ones(16, 2, device="cuda").t()):
+        param.main_grad, ready = buffer, []
+        param._nmb_grad_ready = lambda: ready.append(1)
+        relative_bias_attention(q, k, v, param, 0.125, max_distance=60).backward(dout)
+        torch.testing.assert_close(buffer, want + 1, rtol=1e-6, atol=1e-6)
+        param._nmb_overwrite_next = True
+        relative_bias_attention(q, k, v, param, 0.125, max_distance=60).backward(dout)
+        torch.testing.assert_close(buffer, want, rtol=0, atol=0)
+        assert ready == [1, 1] and param.grad is None
+
+
+def test_other_stream_and_two_calls_at_once():
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention
+
+    sets = [_tensors(1, 400, 400, 4, 4, 64, 32, seed=s) for s in range(2)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(3):
+        for st, (q, k, v, table, dout) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                out = relative_bias_attention(q, k, v, table, 0.125)
+                results.append((out, *torch.autograd.grad(out, (q, k, v, table), dout)))
+    torch.cuda.synchronize()
+    for n, (q, k, v, table, dout) in enumerate(sets):
+        values, bounds, rms = oracle(q, k, v, dout, 0.125, table=table)
+        for got in results[n::2]:
+            check(dict(zip(("out", "dq", "dk", "dv", "dtable"), got)), values, bounds, rms)
+
+
+def test_two_captured_graphs():
+    from nano_megatron_b200.ops import native
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention, window_attention
+
+    native.lib()
+    q, k, v, table, dout = _tensors(2, 300, 300, 4, 2, 64, 32)
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm-up outside of a capture
+        torch.autograd.grad(relative_bias_attention(q, k, v, table, 0.125), (q, k, v, table), dout)
+    torch.cuda.current_stream().wait_stream(side)
+    for n in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = window_attention(q, k, v, 0.125, window=77, sinks=3) if n == 0 else relative_bias_attention(q, k, v, table, 0.125)
+            outs.append((out, *torch.autograd.grad(out, (q, k, v) if n == 0 else (q, k, v, table), dout)))
+        graphs.append(g)
+    for seed in (1, 2):
+        fresh = _tensors(2, 300, 300, 4, 2, 64, 32, seed=seed)
+        with torch.no_grad():
+            for t, f in zip((q, k, v, table, dout), fresh):
+                t.copy_(f)
+        for g in graphs + graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        native.check_status()
+        for n in range(2):
+            values, bounds, rms = oracle(q, k, v, dout, 0.125, **(dict(window=77, sinks=3) if n == 0 else dict(table=table)))
+            check(dict(zip(("out", "dq", "dk", "dv", "dtable"), outs[n])), values, bounds, rms)
+
+
+@pytest.mark.parametrize("sq,skv,d,start", [(1, 1, 64, 0), (37, 37, 96, 0), (130, 200, 128, 70), (300, 300, 64, 0)])
+@pytest.mark.parametrize("buckets", [0, 32])
+def test_nothing_is_written_outside(sq, skv, d, start, buckets):
+    """Outputs inside larger buffers: what lies around them stays as it was."""
+    from nano_megatron_b200.ops import band_attention as ba
+    from nano_megatron_b200.ops import native
+
+    b, hq, hkv, pad = 2, 4, 2, 9
+    q, k, v, table, dout = (None if t is None else t.detach() for t in _tensors(b, sq, skv, hq, hkv, d, buckets))
+    mark = 7.0
+
+    def inside(s, h):
+        big = torch.full((b, s + 2 * pad, h, d), mark, device="cuda", dtype=torch.bfloat16)
+        return big, big[:, pad:pad + s]
+
+    def flat(n):
+        big = torch.full((n + 64,), mark, device="cuda")
+        return big, big[32:32 + n]
+
+    bufs = {n: inside(s, h) for n, s, h in (("o", sq, hq), ("dq", sq, hq), ("dk", skv, hkv), ("dv", skv, hkv))}
+    stats = {n: flat(b * hq * sq) for n in ("m", "l", "delta")}
+    limits = ba._packed_limits(buckets, 128) if buckets else b""
+    lib = native.lib()
+    if buckets:
+        stats["dtable"] = flat(hq * buckets)
+        stats["dtable_part"] = flat(lib.nmb_band_dtable_part(b, hq, sq, buckets))
+    views = {n: t[1] for n, t in {**bufs, **stats}.items()}
+    args = ba._pack(q, k, v, table, limits, 0.125, 50, 3, start, dout=dout, **views)
+    native.check_rc(lib.nmb_band_fwd(args, native.stream_ptr(q.device)), "nmb_band_fwd")
+    native.check_rc(lib.nmb_band_bwd(args, native.stream_ptr(q.device)), "nmb_band_bwd")
+    torch.cuda.synchronize()
+    native.check_status()
+    for n, (big, view) in bufs.items():
+        assert (big[:, :pad] == mark).all() and (big[:, pad + view.shape[1]:] == mark).all(), n
+        assert not (view == mark).all(), n
+    for n, (big, view) in stats.items():
+        assert (big[:32] == mark).all() and (big[-32:] == mark).all(), n
+    values, bounds, rms = oracle(q, k, v, dout, 0.125, window=50, sinks=3, start=start, table=table)
+    check({n: views[n] for n in ("dq", "dk", "dv")} | {"out": views["o"]}, values, bounds, rms)
+
+
+def test_float32_on_the_gpu_takes_the_expression():
+    q, k, v, table, dout = (t.detach().float().requires_grad_(True) for t in _tensors(1, 70, 70, 2, 1, 64, 8))
+    out = _call(q, k, v, table, 0.125, 20, window=30)
+    values, _, _ = oracle(q, k, v, dout, 0.125, window=30, table=table, max_distance=20)
+    torch.testing.assert_close(out.double(), values["out"], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_of_another_device():
+    q, k, v, table, dout = (t.detach().to("cuda:1").requires_grad_(True) for t in _tensors(1, 200, 200, 2, 2, 64, 32))
+    with torch.cuda.device(0):
+        _compare(q, k, v, table, dout)
