@@ -35,11 +35,12 @@ from . import native
 
 MAX_BUCKETS = 128        # sizes of the kernels' table of first distances
 MAX_DISTANCE = 2048
+_MAX_POSITION = 2 ** 30
 _INT_MAX = 2 ** 31 - 1
 
-# BandArgs of csrc/attention_band.cu: eight tensors (pointer and three strides), seven pointers, thirteen whole
+# BandArgs of csrc/attention_band.cu: eight tensors (pointer and three strides), six pointers, thirteen whole
 # numbers, the scale, the table of first distances.
-_ARGS = struct.Struct("P3q" * 8 + "7P" + "13if" + f"{2 * MAX_BUCKETS}s")
+_ARGS = struct.Struct("P3q" * 8 + "6P" + "13if" + f"{2 * MAX_BUCKETS}s")
 _ABSENT = (0, 0, 0, 0)
 
 
@@ -101,17 +102,17 @@ def _ptr(t: Optional[Tensor]) -> int:
 
 
 def _pack(q, k, v, table, limits, scale, window, sinks, start, *, o, dout=None, dq=None, dk=None, dv=None, m=None, l=None,
-          delta=None, dtable=None, dtable_part=None, accumulate=False) -> bytes:
+          scratch=None, dtable=None, accumulate=False) -> bytes:
     b, sq, hq, d = q.shape
     skv, hkv = k.shape[1], k.shape[2]
     tensors = []
     for t in (q, k, v, o, dout, dq, dk, dv):
         tensors += _ABSENT if t is None else _desc(t)
     buckets = 0 if table is None else table.shape[1]
-    return _ARGS.pack(*tensors, _ptr(m), _ptr(l), _ptr(delta), _ptr(table), _ptr(dtable), _ptr(dtable_part),
+    return _ARGS.pack(*tensors, _ptr(m), _ptr(l), _ptr(scratch), _ptr(table), _ptr(dtable),
                       native.status_word(q.device).data_ptr(), int(table is not None and table.dtype == torch.float32),
                       int(dtable is not None and dtable.dtype == torch.float32), int(accumulate), b, hq, hkv, sq, skv, d,
-                      start, min(window, _INT_MAX), min(sinks, skv), buckets, scale, limits)
+                      start, min(window, _MAX_POSITION), min(sinks, skv), buckets, scale, limits)
 
 
 def _band_fwd(q, k, v, table, limits, scale, window, sinks, start):
@@ -138,18 +139,12 @@ def _grad_buffers(q, k, v):
 
 
 def _band_bwd(q, k, v, table, limits, scale, window, sinks, start, out, stats, dout, dtable=None, accumulate=False):
-    b, sq, hq, _ = q.shape
     dq, dk, dv = _grad_buffers(q, k, v)
-    delta = torch.empty((b, hq, sq), dtype=torch.float32, device=q.device)
-    part = None
     lib = native.lib()
-    if dtable is not None:
-        part = torch.empty(lib.nmb_band_dtable_part(b, hq, sq, table.shape[1]), dtype=torch.float32, device=q.device)
-    args = _pack(q, k, v, table, limits, scale, window, sinks, start, o=out, dout=_readable(dout), dq=dq, dk=dk, dv=dv,
-                 m=stats[0], l=stats[1], delta=delta, dtable=dtable, dtable_part=part, accumulate=accumulate)
-    native.check_rc(lib.nmb_band_bwd(args, native.stream_ptr(q.device)), "nmb_band_bwd")
-    if dtable is not None:
-        native.launches += 1
+    common = dict(o=out, dout=_readable(dout), dq=dq, dk=dk, dv=dv, m=stats[0], l=stats[1], dtable=dtable, accumulate=accumulate)
+    head = (q, k, v, table, limits, scale, window, sinks, start)
+    scratch = torch.empty(lib.nmb_band_bwd_scratch(_pack(*head, **common)), dtype=torch.float32, device=q.device)
+    native.check_rc(lib.nmb_band_bwd(_pack(*head, scratch=scratch, **common), native.stream_ptr(q.device)), "nmb_band_bwd")
     return dq, dk, dv
 
 
@@ -231,8 +226,8 @@ def _check(q: Tensor, k: Tensor, v: Tensor, scale: float, window: Optional[int],
     window = _INT_MAX if window is None else _check_int("window", window, 1)
     sinks = _check_int("sinks", sinks, 0)
     start = _check_int("query_start", query_start, 0)
-    if start + q.shape[1] > _INT_MAX // 2 or k.shape[1] > _INT_MAX // 2:
-        raise ValueError(f"positions must stay below {_INT_MAX // 2}; got query_start {start}, q={tuple(q.shape)}, "
+    if start + q.shape[1] > _MAX_POSITION or k.shape[1] > _MAX_POSITION:
+        raise ValueError(f"positions must stay below {_MAX_POSITION}; got query_start {start}, q={tuple(q.shape)}, "
                          f"k={tuple(k.shape)}")
     return scale, window, sinks, start
 

@@ -100,7 +100,8 @@ def lib() -> ctypes.CDLL:
                 _lib = ctypes.CDLL(str(_LIB_PATH))
                 for fn in (_lib.nmb_band_fwd, _lib.nmb_band_bwd):
                     fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]   # packed arguments, stream
-                _lib.nmb_band_dtable_part.restype = ctypes.c_longlong
+                _lib.nmb_band_bwd_scratch.argtypes = [ctypes.c_char_p]
+                _lib.nmb_band_bwd_scratch.restype = ctypes.c_longlong
                 pair = os.environ.get("NMB_GEMM_PAIR")
                 if pair is not None:
                     _lib.nmb_gemm_set_pair(int(pair != "0"))

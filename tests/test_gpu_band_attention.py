@@ -254,13 +254,15 @@ def test_nothing_is_written_outside(sq, skv, d, start, buckets):
         return big, big[32:32 + n]
 
     bufs = {n: inside(s, h) for n, s, h in (("o", sq, hq), ("dq", sq, hq), ("dk", skv, hkv), ("dv", skv, hkv))}
-    stats = {n: flat(b * hq * sq) for n in ("m", "l", "delta")}
+    stats = {n: flat(b * hq * sq) for n in ("m", "l")}
     limits = ba._packed_limits(buckets, 128) if buckets else b""
     lib = native.lib()
     if buckets:
         stats["dtable"] = flat(hq * buckets)
-        stats["dtable_part"] = flat(lib.nmb_band_dtable_part(b, hq, sq, buckets))
     views = {n: t[1] for n, t in {**bufs, **stats}.items()}
+    args = ba._pack(q, k, v, table, limits, 0.125, 50, 3, start, dout=dout, **views)
+    stats["scratch"] = flat(lib.nmb_band_bwd_scratch(args))
+    views["scratch"] = stats["scratch"][1]
     args = ba._pack(q, k, v, table, limits, 0.125, 50, 3, start, dout=dout, **views)
     native.check_rc(lib.nmb_band_fwd(args, native.stream_ptr(q.device)), "nmb_band_fwd")
     native.check_rc(lib.nmb_band_bwd(args, native.stream_ptr(q.device)), "nmb_band_bwd")
