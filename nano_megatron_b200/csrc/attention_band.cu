@@ -20,14 +20,16 @@ constexpr int kMaxBuckets = 128;
 constexpr int kMaxDistance = 2048;
 constexpr float kBiasLimit = 3.0e38f;  // finite biases stay finite after the change to base 2
 
-struct BandTensor {
-  void* ptr;
-  long long stride_b, stride_s, stride_h;  // elements; head_dim is contiguous
+struct BandStride {
+  long long b, s, h;  // elements; head_dim is contiguous
 };
 
-// Arguments of both passes, laid out as in ops/band_attention.py.
+// Arguments of both passes, laid out as in ops/band_attention.py: the pointers of a call, then what its shapes fix.
 struct BandArgs {
-  BandTensor q, k, v, o, dout, dq, dk, dv;
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16* o;
+  const __nv_bfloat16* dout;
+  __nv_bfloat16 *dq, *dk, *dv;
   float* m;              // [B, Hq, Sq]
   float* l;              // [B, Hq, Sq]
   float* scratch;        // nmb_band_bwd_scratch() floats, backward only
@@ -35,9 +37,12 @@ struct BandArgs {
   void* dtable;          // [Hq, buckets]; null when it is not wanted
   int* status;
   int table_fp32, dtable_fp32, accumulate;  // accumulate: dtable is added to
+  int pad;
+  BandStride q_st, k_st, v_st, o_st, dout_st, dq_st, dk_st, dv_st;
   int B, Hq, Hkv, Sq, Skv, d;
   int q_pos0, window, sinks, buckets;
   float scale;
+  int pad2;
   unsigned short limit[kMaxBuckets];  // first distance of bucket b + 1
 };
 
@@ -56,8 +61,9 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ const __nv_bfloat16* band_row(const BandTensor& t, int b, int s, int h) {
-  return static_cast<const __nv_bfloat16*>(t.ptr) + b * t.stride_b + s * t.stride_s + h * t.stride_h;
+template <typename T>
+__device__ __forceinline__ T* band_row(T* ptr, const BandStride& st, int b, int s, int h) {
+  return ptr + b * st.b + s * st.s + h * st.h;
 }
 
 // ------------------------------------------------------------- key tiles --
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
       }
       if (!ok) break;
       const long long stat = (static_cast<long long>(w.b) * a.Hq + h) * a.Sq + row;
-      __nv_bfloat16* out = const_cast<__nv_bfloat16*>(band_row(a.o, w.b, row, h));
+      __nv_bfloat16* out = band_row(a.o, a.o_st, w.b, row, h);
       if (n > 0) {
         if (!warp_wait(&o_full[t], n_item & 1, abort_flag, a.status, 69)) {
           ok = false;
@@ -570,12 +576,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
   }
 }
 
-static int make_band_map(CUtensorMap* m, const BandTensor& t, int d, int S, int H, int B) {
+static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStride& t, int d, int S, int H, int B) {
   const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(S), static_cast<uint64_t>(H), static_cast<uint64_t>(B)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(t.stride_s) * 2, static_cast<uint64_t>(t.stride_h) * 2,
-                               static_cast<uint64_t>(t.stride_b) * 2};
+  const uint64_t strides[3] = {static_cast<uint64_t>(t.s) * 2, static_cast<uint64_t>(t.h) * 2,
+                               static_cast<uint64_t>(t.b) * 2};
   const uint32_t box[4] = {64, 128, 1, 1};
-  return make_tmap_bf16(m, t.ptr, 4, dims, strides, box);
+  return make_tmap_bf16(m, ptr, 4, dims, strides, box);
 }
 
 template <int D>
@@ -873,7 +879,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
       if (n > 0) {
         constexpr int kChunks = D / 16;  // 16-byte chunks of half a row
         uint4 o[kChunks];
-        const uint4* src = reinterpret_cast<const uint4*>(band_row(a.o, w.b, valid ? row : w.q0, w.h)) + half * kChunks;
+        const uint4* src = reinterpret_cast<const uint4*>(band_row(a.o, a.o_st, w.b, valid ? row : w.q0, w.h)) + half * kChunks;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) o[c] = src[c];
         const int qs = n_item % QS;
@@ -1018,7 +1024,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
         }
       }
       if (!ok) break;
-      __nv_bfloat16* out = const_cast<__nv_bfloat16*>(band_row(a.dq, w.b, row, w.h)) + half * (D / 2);
+      __nv_bfloat16* out = band_row(a.dq, a.dq_st, w.b, row, w.h) + half * (D / 2);
       if (n > 0) {
         if (!warp_wait(dq_full, n_item & 1, abort_flag, a.status, 91)) break;
         ++n_item;
@@ -1481,7 +1487,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const float mul = which == 0 ? 1.f : a.scale;
-        __nv_bfloat16* out = const_cast<__nv_bfloat16*>(band_row(which == 0 ? a.dv : a.dk, w.b, j, w.hk)) + half * (D / 2);
+        __nv_bfloat16* out = band_row(which == 0 ? a.dv : a.dk, which == 0 ? a.dv_st : a.dk_st, w.b, j, w.hk) + half * (D / 2);
         float* part = p.part + ((static_cast<long long>(w.slot) * 2 + which) * 128 + r) * D + half * (D / 2);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -1520,10 +1526,32 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
   }
 }
 
-// Sums the pieces of split key tiles, in order: eight values of a row per thread.
-__global__ void band_dkv_sum_kernel(const __grid_constant__ BandBwdParams p) {
+// What is left after them, in one launch.  The first `sum_blocks` blocks add the pieces of split key tiles, in order: eight
+// values of a row per thread.  The others add the table's gradient, over batches and query tiles in a fixed order: a warp per
+// (head, bucket).
+__global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant__ BandBwdParams p, int sum_blocks) {
   pdl_enter();
   const BandArgs& a = p.a;
+  if (static_cast<int>(blockIdx.x) >= sum_blocks) {
+    const int at = (blockIdx.x - sum_blocks) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (at >= a.Hq * a.buckets) return;
+    const int h = at / a.buckets, bucket = at % a.buckets;
+    float acc = 0.f;
+    for (int b = 0; b < a.B; ++b)
+      for (int t = lane; t < p.n_qt; t += 32)
+        acc += p.dtable_part[((static_cast<long long>(b) * a.Hq + h) * p.n_qt + t) * a.buckets + bucket];
+    acc = warp_sum(acc);
+    if (lane == 0) {
+      if (a.dtable_fp32) {
+        float* out = static_cast<float*>(a.dtable) + at;
+        *out = a.accumulate ? *out + acc : acc;
+      } else {
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.dtable) + at;
+        *out = __float2bfloat16(a.accumulate ? __bfloat162float(*out) + acc : acc);
+      }
+    }
+    return;
+  }
   const int n_hb = a.Hkv * a.B, per_row = a.d / 8;
   const int sink_items = p.sink_tiles * p.sink_pieces * n_hb;
   const int first = p.sink_pieces > 1 ? 0 : p.sink_tiles, end = p.pieces > 1 ? p.n_kt : p.sink_tiles;
@@ -1551,36 +1579,10 @@ __global__ void band_dkv_sum_kernel(const __grid_constant__ BandBwdParams p) {
     x[4] += v.x; x[5] += v.y; x[6] += v.z; x[7] += v.w;
   }
   const float mul = which == 0 ? 1.f : a.scale;
-  __nv_bfloat16* out = const_cast<__nv_bfloat16*>(band_row(which == 0 ? a.dv : a.dk, hb / a.Hkv, j, hb % a.Hkv)) + c8 * 8;
+  __nv_bfloat16* out = 
+      band_row(which == 0 ? a.dv : a.dk, which == 0 ? a.dv_st : a.dk_st, hb / a.Hkv, j, hb % a.Hkv) + c8 * 8;
   *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(x[0] * mul, x[1] * mul), pack_bf16x2(x[2] * mul, x[3] * mul),
                                               pack_bf16x2(x[4] * mul, x[5] * mul), pack_bf16x2(x[6] * mul, x[7] * mul));
-}
-
-// dtable[h, b] = sum over batches and query tiles, in a fixed order.
-__global__ void band_dtable_kernel(const __grid_constant__ BandBwdParams p) {
-  pdl_enter();
-  __shared__ float sums[128];
-  const BandArgs& a = p.a;
-  const int h = blockIdx.x / a.buckets, bucket = blockIdx.x % a.buckets;
-  float acc = 0.f;
-  for (int b = 0; b < a.B; ++b)
-    for (int t = threadIdx.x; t < p.n_qt; t += 128)
-      acc += p.dtable_part[((static_cast<long long>(b) * a.Hq + h) * p.n_qt + t) * a.buckets + bucket];
-  sums[threadIdx.x] = acc;
-  __syncthreads();
-  for (int o = 64; o > 0; o >>= 1) {
-    if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    if (a.dtable_fp32) {
-      float* out = static_cast<float*>(a.dtable) + blockIdx.x;
-      *out = a.accumulate ? *out + sums[0] : sums[0];
-    } else {
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.dtable) + blockIdx.x;
-      *out = __float2bfloat16(a.accumulate ? __bfloat162float(*out) + sums[0] : sums[0]);
-    }
-  }
 }
 
 // Steps (query tiles times heads) of a key tile, as in dkv_item.
@@ -1653,13 +1655,12 @@ static cudaError_t launch_band_bwd(BandBwdParams& p, long long dq_items, long lo
   p.n_items = static_cast<int>(dkv_items);
   e = launch_pdl(band_bwd_dkv_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBwdBandThreads),
                  BandDkvSmem<D>::kLut + lut, s, p);
-  if (e == cudaSuccess && split) {
-    const int tiles = (p.pieces > 1 ? p.n_kt : p.sink_tiles) - (p.sink_pieces > 1 ? 0 : p.sink_tiles);
-    const long long octets = static_cast<long long>(tiles) * p.a.Hkv * p.a.B * 2 * 128 * (D / 8);
-    e = launch_pdl(band_dkv_sum_kernel, dim3(static_cast<unsigned>((octets + 255) / 256)), dim3(256), 0, s, p);
-  }
-  if (e == cudaSuccess && p.a.dtable != nullptr)
-    e = launch_pdl(band_dtable_kernel, dim3(p.a.Hq * p.a.buckets), dim3(128), 0, s, p);
+  const int tiles = !split ? 0 : (p.pieces > 1 ? p.n_kt : p.sink_tiles) - (p.sink_pieces > 1 ? 0 : p.sink_tiles);
+  const long long sum_blocks = static_cast<long long>(tiles) * p.a.Hkv * p.a.B * (D / 8);  // 2 * 128 rows of D / 8 octets, 256 a block
+  const int table_blocks = p.a.dtable == nullptr ? 0 : (p.a.Hq * p.a.buckets + 7) / 8;
+  if (e == cudaSuccess && sum_blocks + table_blocks > 0)
+    e = launch_pdl(band_finish_kernel, dim3(static_cast<unsigned>(sum_blocks + table_blocks)), dim3(256), 0, s, p,
+                   static_cast<int>(sum_blocks));
   return e;
 }
 
@@ -1672,13 +1673,14 @@ static int band_check(const BandArgs* a) {
   if (a->B < 1 || a->Hkv < 1 || a->Hq % a->Hkv != 0 || a->Sq < 1 || a->Skv < 1) return kBadArgument;
   if (a->q_pos0 < 0 || a->window < 1 || a->sinks < 0 || !(a->scale > 0.f)) return kBadArgument;
   if (a->table != nullptr && (a->buckets < 2 || a->buckets > kMaxBuckets || a->limit[a->buckets - 2] > kMaxDistance)) return kBadArgument;
-  for (const BandTensor* t : {&a->q, &a->k, &a->v, &a->o, &a->dout, &a->dq, &a->dk, &a->dv}) {
-    const bool written = t == &a->o || t == &a->dq || t == &a->dk || t == &a->dv;  // 32-byte stores
-    const int bytes = written ? 32 : 16;
-    if (reinterpret_cast<uintptr_t>(t->ptr) % bytes != 0 || t->stride_b * 2 % bytes != 0 || t->stride_s * 2 % bytes != 0 ||
-        t->stride_h * 2 % bytes != 0)
-      return kBadArgument;
-  }
+  auto aligned = [](const void* ptr, const BandStride& t, int bytes) {
+    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && t.b * 2 % bytes == 0 && t.s * 2 % bytes == 0 && t.h * 2 % bytes == 0;
+  };
+  // tile loads want 16 bytes; results are written in pieces of 32
+  if (!aligned(a->q, a->q_st, 16) || !aligned(a->k, a->k_st, 16) || !aligned(a->v, a->v_st, 16) || !aligned(a->o, a->o_st, 32) ||
+      !aligned(a->dout, a->dout_st, 16) || !aligned(a->dq, a->dq_st, 32) || !aligned(a->dk, a->dk_st, 32) ||
+      !aligned(a->dv, a->dv_st, 32))
+    return kBadArgument;
   return 0;
 }
 
@@ -1717,9 +1719,9 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   (void)cudaGetLastError();
   BandFwdParams p;
   p.a = *a;
-  if (make_band_map(&p.q_map, a->q, a->d, a->Sq, a->Hq, a->B)) return 101;
-  if (make_band_map(&p.k_map, a->k, a->d, a->Skv, a->Hkv, a->B)) return 102;
-  if (make_band_map(&p.v_map, a->v, a->d, a->Skv, a->Hkv, a->B)) return 103;
+  if (make_band_map(&p.q_map, a->q, a->q_st, a->d, a->Sq, a->Hq, a->B)) return 101;
+  if (make_band_map(&p.k_map, a->k, a->k_st, a->d, a->Skv, a->Hkv, a->B)) return 102;
+  if (make_band_map(&p.v_map, a->v, a->v_st, a->d, a->Skv, a->Hkv, a->B)) return 103;
   p.n_qt = (a->Sq + 127) / 128;
   p.s_pad = p.n_qt * 128;
   p.t_last = a->table == nullptr ? 0 : a->limit[a->buckets - 2];
@@ -1742,10 +1744,10 @@ extern "C" int nmb_band_bwd(const BandArgs* a, void* stream) {
   p.stat = a->scratch;
   p.part = p.stat + w.stat;
   p.dtable_part = p.part + w.part;
-  if (make_band_map(&p.q_map, a->q, a->d, a->Sq, a->Hq, a->B)) return 101;
-  if (make_band_map(&p.k_map, a->k, a->d, a->Skv, a->Hkv, a->B)) return 102;
-  if (make_band_map(&p.v_map, a->v, a->d, a->Skv, a->Hkv, a->B)) return 103;
-  if (make_band_map(&p.do_map, a->dout, a->d, a->Sq, a->Hq, a->B)) return 104;
+  if (make_band_map(&p.q_map, a->q, a->q_st, a->d, a->Sq, a->Hq, a->B)) return 101;
+  if (make_band_map(&p.k_map, a->k, a->k_st, a->d, a->Skv, a->Hkv, a->B)) return 102;
+  if (make_band_map(&p.v_map, a->v, a->v_st, a->d, a->Skv, a->Hkv, a->B)) return 103;
+  if (make_band_map(&p.do_map, a->dout, a->dout_st, a->d, a->Sq, a->Hq, a->B)) return 104;
   const long long n_hb = static_cast<long long>(a->Hkv) * a->B;
   const long long dq_items = static_cast<long long>(p.n_qt) * a->Hq * a->B;
   const long long dkv_items = (static_cast<long long>(p.sink_tiles) * p.sink_pieces +

@@ -43,7 +43,7 @@ _splitk_keep: dict[int, tuple] = {}
 def _configure_current_device(loaded: ctypes.CDLL) -> None:
     """Shared-memory opt-ins of the big kernels are per device: set them the
     first time the library is used with a given device current."""
-    if not torch.cuda.is_available():
+    if not _configured_devices and not torch.cuda.is_available():
         return
     dev = torch.cuda.current_device()
     if dev in _configured_devices:

@@ -255,17 +255,26 @@ def test_nothing_is_written_outside(sq, skv, d, start, buckets):
 
     bufs = {n: inside(s, h) for n, s, h in (("o", sq, hq), ("dq", sq, hq), ("dk", skv, hkv), ("dv", skv, hkv))}
     stats = {n: flat(b * hq * sq) for n in ("m", "l")}
-    limits = ba._packed_limits(buckets, 128) if buckets else b""
     lib = native.lib()
+    p = ba._plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), True, buckets or None, 128, 0.125, 50, 3, start)
     if buckets:
         stats["dtable"] = flat(hq * buckets)
+    stats["scratch"] = flat(ba._scratch(p, lib))
     views = {n: t[1] for n, t in {**bufs, **stats}.items()}
-    args = ba._pack(q, k, v, table, limits, 0.125, 50, 3, start, dout=dout, **views)
-    stats["scratch"] = flat(lib.nmb_band_bwd_scratch(args))
-    views["scratch"] = stats["scratch"][1]
-    args = ba._pack(q, k, v, table, limits, 0.125, 50, 3, start, dout=dout, **views)
-    native.check_rc(lib.nmb_band_fwd(args, native.stream_ptr(q.device)), "nmb_band_fwd")
-    native.check_rc(lib.nmb_band_bwd(args, native.stream_ptr(q.device)), "nmb_band_bwd")
+
+    def at(n):
+        return views[n].data_ptr() if n in views else 0
+
+    # the same strides but for the batch: rows of larger buffers
+    fixed = list(ba._FIXED.unpack(p.bwd))
+    for n, i in (("o", 3), ("dq", 5), ("dk", 6), ("dv", 7)):
+        fixed[3 * i] = views[n].stride(0)
+    args = ba._POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), at("o"), dout.data_ptr(), at("dq"), at("dk"), at("dv"), at("m"),
+                             at("l"), at("scratch"), 0 if table is None else table.data_ptr(), at("dtable"),
+                             native.status_word(q.device).data_ptr(), 0, 1, 0, 0) + ba._FIXED.pack(*fixed)
+    stream = torch.cuda.current_stream().cuda_stream
+    native.check_rc(lib.nmb_band_fwd(args, stream), "nmb_band_fwd")
+    native.check_rc(lib.nmb_band_bwd(args, stream), "nmb_band_bwd")
     torch.cuda.synchronize()
     native.check_status()
     for n, (big, view) in bufs.items():
