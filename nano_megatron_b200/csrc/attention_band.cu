@@ -122,17 +122,69 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// D[tmem] (+)= A[tmem, 128 rows of bf16 pairs] * B[smem]
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                               uint32_t accumulate) {
+// The issuing warp runs its loops with all lanes together and lets one lane of them issue: addresses then are the same for
+// the whole warp by construction, which is where the instruction wants them (uniform registers).  With the loops inside a
+// branch of one lane every operand was moved there first and issuing, not the tensor core, set the pace (a step of two slots
+// at d = 128: 4160 clocks to issue 32 products that take 2048).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(e));
+  return e != 0;
+}
+// Shared-memory operands: the low word of a descriptor (address and the stride between slabs of an MN-major operand) moves
+// from product to product, the high word does not.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row stride 1024, version, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_k(uint32_t smem) { return ((smem & 0x3ffff) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t smem) { return ((smem & 0x3ffff) >> 4) | ((16384u >> 4) << 16); }
+
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+      "}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "n"(kAccumulate ? 1 : 0), "n"(kDescHigh)
       : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+      "}" ::"r"(d),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+// D[128 x 128] = A B^T over a depth of D, both K-major; one lane
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc) {
+  mma_ss<false>(d, a_low, b_low, idesc);
+#pragma unroll
+  for (int k = 1; k < D / 16; ++k) {
+    const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+    mma_ss<true>(d, a_low + off, b_low + off, idesc);
+  }
+}
+// D[128 x n] (+)= A B over a depth of 128, A bf16 in tensor memory (its halves kHalf columns apart), B MN-major; one lane
+template <int kHalf>
+__device__ __forceinline__ void mma_apply(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, bool first) {
+  mma_ts(d, a_tmem, b_low, idesc, first ? 0u : 1u);
+#pragma unroll
+  for (int k = 1; k < 8; ++k) mma_ts(d, a_tmem + (k >> 2) * kHalf + (k & 3) * 8, b_low + k * (2048 >> 4), idesc, 1u);
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -347,12 +399,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
       }
     }
     } else if (warp == 9) {
-    // ---------------------------------------------------------- MMA issuer --
-    if (lane == 0) {
+      // -------------------------------------------------------- MMA issuer --
       constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(128, D, false, true);
       const uint32_t ring = smem_u32(smem + L::kRing);
-      int base = 0, n_p[2] = {0, 0}, n_item[2] = {0, 0};
+      const bool one = elect_one();
+      uint32_t base = 0;
+      uint32_t n_p[2] = {0, 0}, n_item[2] = {0, 0};
       bool ok = true;
       for (int round = 0; ok; ++round) {
         const int item = item_of_round(round);
@@ -361,61 +414,66 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
         const FwdItem w = fwd_item(p, item);
         const int n = w.all.count();
         int left[2] = {w.t[0].count(), w.t[1].count()};
-        bool pending[2] = {false, false}, fresh[2] = {true, true}, any[2] = {left[0] > 0, left[1] > 0};
+        bool pending[2] = {false, false}, fresh[2] = {true, true};
+        const bool any[2] = {left[0] > 0, left[1] > 0};
         // O += P V of tile u for slot t
         auto pv = [&](int t, int u) {
-          const int pos = base + 2 * u + 1;
-          if (!mbar_wait(&kv_full[pos % ST], (pos / ST) & 1, abort_flag, a.status, 63)) return false;
-          if (fresh[t] && n_item[t] > 0 && !mbar_wait(&o_empty[t], (n_item[t] - 1) & 1, abort_flag, a.status, 64)) return false;
-          if (!mbar_wait(&p_full[t], n_p[t] & 1, abort_flag, a.status, 65)) return false;
+          const uint32_t pos = base + 2 * u + 1;
+          if (!warp_wait(&kv_full[pos % ST], (pos / ST) & 1, abort_flag, a.status, 63)) return false;
+          if (fresh[t] && n_item[t] > 0 && !warp_wait(&o_empty[t], (n_item[t] - 1) & 1, abort_flag, a.status, 64)) return false;
+          if (!warp_wait(&p_full[t], n_p[t] & 1, abort_flag, a.status, 65)) return false;
           ++n_p[t];
           tc_fence_after();
-          const uint32_t sv = ring + (pos % ST) * L::kTile;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            tc_mma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, make_smem_desc(sv + k * 2048, 16384, 1024), idesc_o,
-                           (fresh[t] && k == 0) ? 0u : 1u);
+          const uint32_t b_low = desc_mn(ring + (pos % ST) * L::kTile);
+          const bool last = left[t] == 0, first = fresh[t];
+          if (one) {
+            mma_apply<32>(tmem + 256 + t * D, tmem + t * 128, b_low, idesc_o, first);
+            if (last) tc_commit(&o_full[t]);
+          }
           fresh[t] = false;
           pending[t] = false;
-          if (left[t] == 0) tc_commit(&o_full[t]);
           return true;
         };
         for (int u = 0; u < n && ok; ++u) {
-          const int j = tile_at(w.all, u), pos = base + 2 * u;
-          if (!mbar_wait(&kv_full[pos % ST], (pos / ST) & 1, abort_flag, a.status, 66)) {
+          const int j = tile_at(w.all, u);
+          const uint32_t pos = base + 2 * u;
+          if (!warp_wait(&kv_full[pos % ST], (pos / ST) & 1, abort_flag, a.status, 66)) {
             ok = false;
             break;
           }
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (pending[t]) ok = pv(t, u - 1);
-            if (!ok || !w.t[t].uses(j)) continue;
-            if (fresh[t] && !pending[t] && !mbar_wait(&q_full[t], n_item[t] & 1, abort_flag, a.status, 67)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t sk = ring + (pos % ST) * L::kTile, sq = smem_u32(smem + L::kQ + t * L::kTile);
+          const uint32_t b_low = desc_k(ring + (pos % ST) * L::kTile);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-              tc_mma_bf16(tmem + t * 128, make_smem_desc(sq + off, 16, 1024), make_smem_desc(sk + off, 16, 1024), idesc_s,
-                          k != 0 ? 1u : 0u);
+          for (int t = 0; t < 2; ++t) {
+            if (ok && pending[t]) ok = pv(t, u - 1);
+            if (ok && w.t[t].uses(j)) {
+              // the first scores of an item (nothing was multiplied with V since) wait for its queries
+              if (fresh[t] && !pending[t] && !warp_wait(&q_full[t], n_item[t] & 1, abort_flag, a.status, 67)) {
+                ok = false;
+              } else {
+                tc_fence_after();
+                const bool last = --left[t] == 0;
+                if (one) {
+                  mma_scores<D>(tmem + t * 128, desc_k(smem_u32(smem + L::kQ + t * L::kTile)), b_low, idesc_s);
+                  tc_commit(&s_full[t]);
+                  if (last) tc_commit(&q_empty[t]);
+                }
+                pending[t] = true;
+              }
             }
-            tc_commit(&s_full[t]);
-            pending[t] = true;
-            if (--left[t] == 0) tc_commit(&q_empty[t]);
           }
-          if (!ok) break;
-          tc_commit(&kv_empty[pos % ST]);
-          if (u > 0) tc_commit(&kv_empty[(pos - 1) % ST]);
+          if (ok && one) {
+            tc_commit(&kv_empty[pos % ST]);
+            if (u > 0) tc_commit(&kv_empty[(pos - 1) % ST]);
+          }
         }
-        for (int t = 0; t < 2 && ok; ++t)
-          if (pending[t]) ok = pv(t, n - 1);
-        if (ok && n > 0) tc_commit(&kv_empty[(base + 2 * n - 1) % ST]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && pending[t]) ok = pv(t, n - 1);
+        if (ok && n > 0 && one) tc_commit(&kv_empty[(base + 2 * n - 1) % ST]);
         base += 2 * n;
+#pragma unroll
         for (int t = 0; t < 2; ++t) n_item[t] += any[t];
       }
-    }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -779,61 +837,52 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
                         j * 128, w.hk, w.b);
         }
       }
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
       // -------------------------------------------------------- MMA issuer --
       constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t idesc_dq = make_idesc_bf16(128, D, false, true);
       const uint32_t ring = smem_u32(smem + L::kRing);
-      int step = 0, n_item = 0;       // tiles and items begun
+      const bool one = elect_one();
+      uint32_t step = 0, n_item = 0;  // tiles and items begun
       bool prev_first = false, prev_last = false;
+      uint32_t prev_item = 0;
       bool ok = true;
       // dQ += dS K of step s
-      auto issue_dq = [&](int s, bool first, bool last, int item_no) {
-        if (first && item_no > 0 && !mbar_wait(dq_empty, (item_no - 1) & 1, abort_flag, a.status, 83)) return false;
-        if (!mbar_wait(ds_full, s & 1, abort_flag, a.status, 84)) return false;
+      auto issue_dq = [&](uint32_t s, bool first, bool last, uint32_t item_no) {
+        if (first && item_no > 0 && !warp_wait(dq_empty, (item_no - 1) & 1, abort_flag, a.status, 83)) return false;
+        if (!warp_wait(ds_full, s & 1, abort_flag, a.status, 84)) return false;
         tc_fence_after();
-        const int pos = 2 * s;
-        const uint32_t sk = ring + (pos % ST) * L::kTile;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          tc_mma_bf16_ts(tmem + kDq, tmem + kDs + (s & 1) * 64 + k * 8, make_smem_desc(sk + k * 2048, 16384, 1024), idesc_dq,
-                         (first && k == 0) ? 0u : 1u);
-        tc_commit(&kv_empty[pos % ST]);
-        if (last) tc_commit(dq_full);
+        const uint32_t st = 2 * s % ST;
+        if (one) {
+          mma_apply<32>(tmem + kDq, tmem + kDs + (s & 1) * 64, desc_mn(ring + st * L::kTile), idesc_dq, first);
+          tc_commit(&kv_empty[st]);
+          if (last) tc_commit(dq_full);
+        }
         return true;
       };
-      int prev_item = 0;
       for (int round = 0; round < rounds && ok; ++round) {
         const int item = item_of_round(round);
         if (item >= p.n_items) continue;
         const DqItem w = dq_item(p, item);
         const int n = w.t.count();
         if (n == 0) continue;
-        const int qs = n_item % QS;
+        const uint32_t qs = n_item % QS;
+        const uint32_t q_low = desc_k(smem_u32(smem + L::kQ + 2 * qs * L::kTile));
         for (int u = 0; u < n; ++u, ++step) {
-          const int pk = 2 * step, pv = pk + 1;
-          ok = (u > 0 || mbar_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 85)) &&
-               mbar_wait(&kv_full[pk % ST], (pk / ST) & 1, abort_flag, a.status, 86) &&
-               mbar_wait(&kv_full[pv % ST], (pv / ST) & 1, abort_flag, a.status, 87) &&
-               (step == 0 || mbar_wait(sdp_read, (step - 1) & 1, abort_flag, a.status, 88));
+          const uint32_t pk = 2 * step, pv = pk + 1;
+          ok = (u > 0 || warp_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 85)) &&
+               warp_wait(&kv_full[pk % ST], (pk / ST) & 1, abort_flag, a.status, 86) &&
+               warp_wait(&kv_full[pv % ST], (pv / ST) & 1, abort_flag, a.status, 87) &&
+               (step == 0 || warp_wait(sdp_read, (step - 1) & 1, abort_flag, a.status, 88));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sq = smem_u32(smem + L::kQ + 2 * qs * L::kTile), sdo = sq + L::kTile;
-          const uint32_t sk = ring + (pk % ST) * L::kTile, sv = ring + (pv % ST) * L::kTile;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            tc_mma_bf16(tmem, make_smem_desc(sq + off, 16, 1024), make_smem_desc(sk + off, 16, 1024), idesc_s, k != 0 ? 1u : 0u);
+          if (one) {
+            mma_scores<D>(tmem, q_low, desc_k(ring + (pk % ST) * L::kTile), idesc_s);
+            mma_scores<D>(tmem + kDp, q_low + (L::kTile >> 4), desc_k(ring + (pv % ST) * L::kTile), idesc_s);
+            tc_commit(sdp_full);
+            tc_commit(&kv_empty[pv % ST]);
+            if (u == n - 1) tc_commit(&q_empty[qs]);
           }
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            tc_mma_bf16(tmem + kDp, make_smem_desc(sdo + off, 16, 1024), make_smem_desc(sv + off, 16, 1024), idesc_s,
-                        k != 0 ? 1u : 0u);
-          }
-          tc_commit(sdp_full);
-          tc_commit(&kv_empty[pv % ST]);
-          if (u == n - 1) tc_commit(&q_empty[qs]);
           if (step > 0) ok = issue_dq(step - 1, prev_first, prev_last, prev_item);
           if (!ok) break;
           prev_first = u == 0;
@@ -1261,77 +1310,73 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
         bulk_load(smem + L::kStat + st * kStatBlock * 4,
                   p.stat + ((static_cast<long long>(x.w.b) * a.Hq + h) * p.n_qt + qt) * kStatBlock, stat_bytes, &q_full[st]);
       }
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
       // -------------------------------------------------------- MMA issuer --
       constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t idesc_d = make_idesc_bf16(128, D, false, true);
-      const uint32_t sk = smem_u32(smem + L::kK), sv = sk + L::kTile;
-      auto q_at = [&](int n) { return smem_u32(smem + L::kRing + 2 * (n % ST) * L::kTile); };
-      // [128 x 128] = A B^T, both K-major
-      auto scores = [&](uint32_t d, uint32_t sa, uint32_t sb) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          tc_mma_bf16(tmem + d, make_smem_desc(sa + off, 16, 1024), make_smem_desc(sb + off, 16, 1024), idesc_s, k != 0 ? 1u : 0u);
-        }
-      };
-      auto grads = [&](uint32_t d, uint32_t at, uint32_t sb, bool first) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          tc_mma_bf16_ts(tmem + d, tmem + at + (k >> 2) * kHalf + (k & 3) * 8, make_smem_desc(sb + k * 2048, 16384, 1024), idesc_d,
-                         (first && k == 0) ? 0u : 1u);
-      };
+      const uint32_t sk = smem_u32(smem + L::kK), ring = smem_u32(smem + L::kRing);
+      const uint32_t k_low = desc_k(sk), v_low = desc_k(sk + L::kTile);
+      const bool one = elect_one();
       DkvWalk x;
-      int n = 0, n_item = 0;  // step, item of `x`
+      uint32_t n = 0, n_item = 0;  // step, item of `x`
       bool more = x.open(p, 0);
-      bool ok = more && mbar_wait(kv_full, 0, abort_flag, a.status, 103) && mbar_wait(&q_full[0], 0, abort_flag, a.status, 104);
+      bool ok = more && warp_wait(kv_full, 0, abort_flag, a.status, 103) && warp_wait(&q_full[0], 0, abort_flag, a.status, 104);
       if (ok) {
         tc_fence_after();
-        scores(0, sk, q_at(0));
-        tc_commit(s_full);
-        scores(kDp, sv, q_at(0) + L::kTile);
-        tc_commit(dp_full);
-        if (x.last()) tc_commit(kv_empty);
+        const bool last = x.last();
+        if (one) {
+          mma_scores<D>(tmem, k_low, desc_k(ring), idesc_s);
+          tc_commit(s_full);
+          mma_scores<D>(tmem + kDp, v_low, desc_k(ring + L::kTile), idesc_s);
+          tc_commit(dp_full);
+          if (last) tc_commit(kv_empty);
+        }
       }
       while (ok && more) {
         DkvWalk y = x;
-        const bool ahead = y.next(p), fresh = ahead && y.first();
-        const int n_item2 = n_item + fresh;
-        const uint32_t sq = q_at(n), sq2 = q_at(n + 1);
-        // S^T of the next step
+        const bool ahead = y.next(p), fresh = ahead && y.first(), y_last = ahead && y.last();
+        const bool x_first = x.first(), x_last = x.last();
+        const uint32_t n_item2 = n_item + fresh;
+        const uint32_t sq = ring + 2 * (n % ST) * L::kTile, sq2 = ring + 2 * ((n + 1) % ST) * L::kTile;
+        // S^T and dP^T of the next step
         auto next_s = [&]() {
           if (!ahead) return true;
-          if (fresh && !mbar_wait(kv_full, n_item2 & 1, abort_flag, a.status, 105)) return false;
-          if (!mbar_wait(&q_full[(n + 1) % ST], ((n + 1) / ST) & 1, abort_flag, a.status, 106)) return false;
-          if (kOwn && !mbar_wait(s_read, n & 1, abort_flag, a.status, 107)) return false;
+          if (fresh && !warp_wait(kv_full, n_item2 & 1, abort_flag, a.status, 105)) return false;
+          if (!warp_wait(&q_full[(n + 1) % ST], ((n + 1) / ST) & 1, abort_flag, a.status, 106)) return false;
+          if (kOwn && !warp_wait(s_read, n & 1, abort_flag, a.status, 107)) return false;
           tc_fence_after();
-          scores(0, sk, sq2);
-          tc_commit(s_full);
+          if (one) {
+            mma_scores<D>(tmem, k_low, desc_k(sq2), idesc_s);
+            tc_commit(s_full);
+          }
           return true;
         };
+        auto next_dp = [&]() {
+          if (one) {
+            mma_scores<D>(tmem + kDp, v_low, desc_k(sq2 + L::kTile), idesc_s);
+            tc_commit(dp_full);
+            if (y_last) tc_commit(kv_empty);
+          }
+        };
         if (kOwn && !next_s()) break;
-        if (x.first() && n_item > 0 && !mbar_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
-        if (!mbar_wait(p_full, n & 1, abort_flag, a.status, 109)) break;
+        if (x_first && n_item > 0 && !warp_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
+        if (!warp_wait(p_full, n & 1, abort_flag, a.status, 109)) break;
         tc_fence_after();
-        grads(kDv, kP, sq + L::kTile, x.first());
+        if (one) mma_apply<kHalf>(tmem + kDv, tmem + kP, desc_mn(sq + L::kTile), idesc_d, x_first);
         if (!kOwn && !next_s()) break;
         if (kOwn && ahead) {
-          if (!mbar_wait(dp_read, n & 1, abort_flag, a.status, 110)) break;
+          if (!warp_wait(dp_read, n & 1, abort_flag, a.status, 110)) break;
           tc_fence_after();
-          scores(kDp, sv, sq2 + L::kTile);
-          tc_commit(dp_full);
-          if (y.last()) tc_commit(kv_empty);
+          next_dp();
         }
-        if (!mbar_wait(ds_full, n & 1, abort_flag, a.status, 111)) break;
+        if (!warp_wait(ds_full, n & 1, abort_flag, a.status, 111)) break;
         tc_fence_after();
-        grads(kDk, kDs, sq, x.first());
-        tc_commit(&q_empty[n % ST]);
-        if (x.last()) tc_commit(acc_full);
-        if (!kOwn && ahead) {
-          scores(kDp, sv, sq2 + L::kTile);
-          tc_commit(dp_full);
-          if (y.last()) tc_commit(kv_empty);
+        if (one) {
+          mma_apply<kHalf>(tmem + kDk, tmem + kDs, desc_mn(sq), idesc_d, x_first);
+          tc_commit(&q_empty[n % ST]);
+          if (x_last) tc_commit(acc_full);
         }
+        if (!kOwn && ahead) next_dp();
         x = y;
         more = ahead;
         n_item = n_item2;
