@@ -179,17 +179,93 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_low, uint32_t 
     mma_ss<true>(d, a_low + off, b_low + off, idesc);
   }
 }
-// D[128 x n] (+)= A B over a depth of 128, A bf16 in tensor memory (its halves kHalf columns apart), B MN-major; one lane
-template <int kHalf>
+// D[128 x n] (+)= A B over a depth of 16 kSteps, A bf16 in tensor memory (kPer steps side by side, the next kStride columns
+// on), B MN-major; one lane
+template <int kSteps, int kPer, int kStride>
 __device__ __forceinline__ void mma_apply(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, bool first) {
   mma_ts(d, a_tmem, b_low, idesc, first ? 0u : 1u);
 #pragma unroll
-  for (int k = 1; k < 8; ++k) mma_ts(d, a_tmem + (k >> 2) * kHalf + (k & 3) * 8, b_low + k * (2048 >> 4), idesc, 1u);
+  for (int k = 1; k < kSteps; ++k) mma_ts(d, a_tmem + (k / kPer) * kStride + (k % kPer) * 8, b_low + k * (2048 >> 4), idesc, 1u);
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x for two x, on the FMA pipe: x = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves it in the low bits), 2^f
+// by the polynomial of degree 4 with the smallest relative error on [-1/2, 1/2] (2.7e-6, found by exchange of extrema), 2^n
+// added to the exponent.  x below -126 gives 2^-126.  The exponential unit does 16 a clock and SM, a tile of 128 x 128 weights
+// 1024 clocks, as long as the tensor core takes for its products at d = 128; a part of the weights goes this way instead.
+__device__ __forceinline__ void exp2_pair_fma(uint64_t x2, float& y0, float& y1) {
+  float x0, x1;
+  unpack2(x2, x0, x1);
+  const uint64_t x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t t = add2(x, pack2(12582912.f, 12582912.f));
+  const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
+  uint64_t q = fma2(f, pack2(9.570102207362652e-3f, 9.570102207362652e-3f), pack2(5.591785907745361e-2f, 5.591785907745361e-2f));
+  q = fma2(q, f, pack2(0.240247443318367f, 0.240247443318367f));
+  q = fma2(q, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  q = fma2(q, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1, q0, q1;
+  unpack2(t, t0, t1);
+  unpack2(q, q0, q1);
+  y0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
+  y1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
+}
+// One pair in this many takes that way.
+#ifndef NMB_FMA_PAIRS
+#define NMB_FMA_PAIRS 4
+#endif
+constexpr int kFmaPairs = NMB_FMA_PAIRS;
+template <bool kMix>
+__device__ __forceinline__ void exp2_pair(int pair, uint64_t x2, float& y0, float& y1) {
+  if (kMix && (pair % kFmaPairs) == kFmaPairs - 1) {
+    exp2_pair_fma(x2, y0, y1);
+  } else {
+    float x0, x1;
+    unpack2(x2, x0, x1);
+    y0 = ex2(x0);
+    y1 = ex2(x1);
+  }
+}
+// Weights 2^(s * mul + shift) of 32 scores, as bf16 pairs, and their sum.
+template <bool kMix>
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t mul, uint64_t shift, uint64_t& sum, uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    float p0, p1;
+    exp2_pair<kMix>(k, fma2(pack2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), mul, shift), p0, p1);
+    sum = add2(sum, pack2(p0, p1));
+    pk[k] = pack_bf16x2(p0, p1);
+  }
 }
 // 32 bytes to a 32-byte aligned address: a whole sector per lane
 __device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
@@ -198,28 +274,104 @@ __device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, ui
                "r"(f), "r"(g), "r"(h)
                : "memory");
 }
-// 32 consecutive values of a row as bf16
-__device__ __forceinline__ void store_bf16_32(__nv_bfloat16* dst, const uint32_t (&r)[32], float mul) {
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 consecutive values of a row as bf16
+__device__ __forceinline__ void store_bf16_16(__nv_bfloat16* dst, const uint32_t (&r)[16], float mul) {
+  uint32_t w[8];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    uint32_t w[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      w[k] = pack_bf16x2(__uint_as_float(r[q * 16 + 2 * k]) * mul, __uint_as_float(r[q * 16 + 2 * k + 1]) * mul);
-    st_global_32(dst + q * 16, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+  for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(__uint_as_float(r[2 * k]) * mul, __uint_as_float(r[2 * k + 1]) * mul);
+  st_global_32(dst, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+}
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// Bounded wait: as mbar_wait, but asleep for up to kNapNs at a time after the first look.  (Even a wait that is satisfied
+// takes about 150 clocks; what a role waits for is ordered so that the awaited thing comes last.)
+constexpr uint32_t kNapNs = 10000;
+__device__ __forceinline__ bool band_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kNapNs)
+        : "memory");
+    if (done != 0) return true;
+    if (*abort_flag != 0) return false;
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      report_status(status, kMbarTimeout, where);
+      *abort_flag = 1;
+      return false;
+    }
   }
 }
-// A wait of a whole warp: the same answer in every lane, so that the warp stays together for .aligned instructions.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where));
+// Several at once: their latencies overlap.
+struct BandBar {
+  uint64_t* bar;
+  uint32_t parity;
+};
+__device__ __forceinline__ bool try_wait_all(const BandBar& a, const BandBar& b) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(smem_u32(a.bar)), "r"(a.parity), "r"(smem_u32(b.bar)), "r"(b.parity)
+      : "memory");
+  return ok != 0;
 }
-// All warps that `bar` counts; like every wait, it ends when another role gave up.
-__device__ __forceinline__ bool group_sync(uint64_t* bar, uint32_t& phase, volatile int* abort_flag, int* status, int where) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-  const bool ok = warp_wait(bar, phase, abort_flag, status, where);
-  phase ^= 1;
-  return ok;
+__device__ __forceinline__ bool try_wait_all(const BandBar& a, const BandBar& b, const BandBar& c) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q, r;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "and.pred p, p, q;\n\t"
+      "and.pred p, p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(smem_u32(a.bar)), "r"(a.parity), "r"(smem_u32(b.bar)), "r"(b.parity), "r"(smem_u32(c.bar)), "r"(c.parity)
+      : "memory");
+  return ok != 0;
+}
+template <typename... Bars>
+__device__ __forceinline__ bool band_wait_all(volatile int* abort_flag, int* status, int where, const Bars&... bars) {
+  if (try_wait_all(bars...)) return true;
+  return (band_wait(bars.bar, bars.parity, abort_flag, status, where) && ...);
+}
+// The compute warps' waits.  After one has failed the others are passed by and the loops run to their end on whatever is
+// there: every warp comes to every named barrier, whichever of them gave up, and no warp waits at one for another that left.
+#define NMB_BAND_WAIT(bar, parity, where)                                            \
+  do {                                                                               \
+    ok = ok && band_wait(bar, parity, abort_flag, a.status, where);                  \
+    __syncwarp();                                                                    \
+  } while (0)
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // Items are sorted longest first; rounds alternate in direction so that no CTA gets the longest of every round.
@@ -231,14 +383,23 @@ __device__ __forceinline__ int item_of_round(int round) {
 // ---------------------------------------------------------------- forward --
 // A CTA works on two query tiles ("slots") at a time against the same key tiles: two heads of a group where the group is
 // even, else two neighbouring tiles of a head, else (few tiles in all) one.  While the softmax warps of one slot turn its
-// scores into weights the tensor core works on the other's.  384 threads:
-//   warps 0-3, 4-7  softmax of slot 0, 1: a thread per query row
-//   warp 8          TMA producer: Q per slot, K and V tiles in one ring
-//   warp 9          TMEM owner, tcgen05.mma issuer
-// TMEM: S of the slots at columns 0 and 128, O at 256 and 256 + D.  P (bf16) overwrites the first 64 columns of its S
-// and is the A operand of P V from there.  The CTA stays for all its items: loads and the first products of the next item
-// run under the last steps of the one before.
-constexpr int kFwdThreads = 384;  // whole warpgroups: registers are handed from the last one to the first two
+// scores into weights the tensor core works on the other's.  640 threads:
+//   warps 0-7, 8-15  softmax of slot 0, 1: two threads per query row, 64 keys each, that agree on the maximum through shared
+//                    memory.  One thread per row left two warps per scheduler, whose latencies nothing covered.
+//   warp 16          TMA producer: Q per slot, K and V tiles in one ring
+//   warps 17, 18     tcgen05.mma issuers.  At D = 64 one per slot: with one for both, each wait of one slot kept the other's
+//                    products back.  At D > 64 the tensor core is what is scarce and one issues for both: products of two
+//                    issuers take turns one by one, both slots then wait for them and work on weights at the same time, and
+//                    nothing overlaps (326 against 265 us, 8192 positions, 16 heads of 128)
+// TMEM: S of the slots at columns 0 and 128, O at 256 and 256 + D.  P (bf16), the A operand of P V, has columns of its own
+// where there is room (D = 64: 384, 448): the next scores are then computed while this tile's weights are.  Else each half
+// overwrites its own part of S.
+// The CTA stays for all its items: loads and the first products of the next item run under the last steps of the one before.
+constexpr int kBandThreads = 640;  // whole warpgroups: registers are handed from the last one to the others
+constexpr int kComputeWarps = 16, kLoadWarp = 16, kMmaWarp = 17;  // kMmaWarp owns the TMEM; it and the next one issue
+// 640 threads start with 96 registers each: 4 * 104 + 56 <= 5 * 96
+#define NMB_BAND_FEW_REGISTERS asm volatile("setmaxnreg.dec.sync.aligned.u32 56;")
+#define NMB_BAND_MORE_REGISTERS asm volatile("setmaxnreg.inc.sync.aligned.u32 104;")
 
 struct BandFwdParams {
   CUtensorMap q_map, k_map, v_map;
@@ -258,8 +419,9 @@ struct BandFwdSmem {
   static constexpr int kQ = 0;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBar = kRing + kStages * kTile;
-  static constexpr int kNumBars = 2 * kStages + 14;
-  static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [2][entries], then the map
+  static constexpr int kNumBars = 2 * kStages + 16;
+  static constexpr int kXch = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [2][2 slots][2 halves][128]
+  static constexpr int kLut = kXch + 4096;                                     // float [2][entries], then the map
 };
 
 struct FwdItem {
@@ -299,9 +461,11 @@ __device__ __forceinline__ FwdItem fwd_item(const BandFwdParams& p, int item) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_constant__ BandFwdParams p) {
+__global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_constant__ BandFwdParams p) {
   using L = BandFwdSmem<D>;
   constexpr int NS = L::kSlabs, ST = L::kStages;
+  constexpr bool kOwn = D == 64;  // P has its own columns
+  constexpr int kIssuers = kOwn ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* kv_full = bars;              // [ST]
@@ -312,7 +476,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
   uint64_t* p_full = q_full + 6;
   uint64_t* o_full = q_full + 8;
   uint64_t* o_empty = q_full + 10;
-  uint64_t* sync_bar = q_full + 12;
+  uint64_t* s_read = q_full + 12;        // only with P's own columns, as the next
+  uint64_t* pv_done = q_full + 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const BandArgs& a = p.a;
@@ -328,35 +493,39 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], kIssuers);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_full[t], 1);
-      mbar_init(&o_empty[t], 4);
-      mbar_init(&sync_bar[t], 4);
+      mbar_init(&o_empty[t], 8);
+      mbar_init(&s_read[t], 8);
+      mbar_init(&pv_done[t], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (a.table != nullptr) build_bucket_map(a, p.t_last, map, threadIdx.x, kFwdThreads);
+  if (a.table != nullptr) build_bucket_map(a, p.t_last, map, threadIdx.x, kBandThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // All 512 columns were allocated, so they begin at 0; said as a constant the addresses need no moves to uniform registers.
+  constexpr uint32_t tmem = 0;
+  if (threadIdx.x == 0 && *tmem_slot != 0) {
+    report_status(a.status, kBadArgument, 75);
+    *abort_flag = 1;
+  }
   pdl_enter();  // the set-up above touches no global memory
-  // 384 threads start with 168 registers each: 2 * 208 + 80 <= 3 * 168
-
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8) {
+  if (warp >= kComputeWarps) {
+    NMB_BAND_FEW_REGISTERS;
+    if (warp == kLoadWarp) {
     // ------------------------------------------------------------ producer --
     if (lane == 0) {
       tma_prefetch_desc(&p.q_map);
@@ -371,7 +540,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
         const FwdItem w = fwd_item(p, item);
         auto load = [&](const CUtensorMap* m, int j) {
           const int st = pos % ST, use = pos / ST;
-          if (use > 0 && !mbar_wait(&kv_empty[st], (use - 1) & 1, abort_flag, a.status, 61)) return false;
+          if (use > 0 && !band_wait(&kv_empty[st], (use - 1) & 1, abort_flag, a.status, 61)) return false;
           mbar_expect_tx(&kv_full[st], L::kTile);
 #pragma unroll
           for (int c = 0; c < NS; ++c)
@@ -382,7 +551,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
         const int n = w.all.count();
         for (int t = 0; t < 2 && ok; ++t) {
           if (w.t[t].count() == 0) continue;
-          if (n_q[t] > 0 && !mbar_wait(&q_empty[t], (n_q[t] - 1) & 1, abort_flag, a.status, 62)) {
+          if (n_q[t] > 0 && !band_wait(&q_empty[t], (n_q[t] - 1) & 1, abort_flag, a.status, 62)) {
             ok = false;
             break;
           }
@@ -398,14 +567,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
         }
       }
     }
-    } else if (warp == 9) {
-      // -------------------------------------------------------- MMA issuer --
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + kIssuers) {
+      // ------------------------------------------------------- MMA issuers --
       constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(128, D, false, true);
+      constexpr int kMine = 2 / kIssuers;  // slots of an issuer
       const uint32_t ring = smem_u32(smem + L::kRing);
+      const int t0 = kOwn ? warp - kMmaWarp : 0;
       const bool one = elect_one();
-      uint32_t base = 0;
-      uint32_t n_p[2] = {0, 0}, n_item[2] = {0, 0};
+      uint32_t base = 0, n_s[kMine] = {}, n_p[kMine] = {}, n_item[kMine] = {};
       bool ok = true;
       for (int round = 0; ok; ++round) {
         const int item = item_of_round(round);
@@ -413,210 +583,292 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
         if (item >= p.n_items) continue;
         const FwdItem w = fwd_item(p, item);
         const int n = w.all.count();
-        int left[2] = {w.t[0].count(), w.t[1].count()};
-        bool pending[2] = {false, false}, fresh[2] = {true, true};
-        const bool any[2] = {left[0] > 0, left[1] > 0};
-        // O += P V of tile u for slot t
-        auto pv = [&](int t, int u) {
+        KeyTiles mine[kMine];
+        int left[kMine];
+        bool any[kMine], pending[kMine], first_s[kMine], first_pv[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          mine[i] = t0 + i == 0 ? w.t[0] : w.t[1];
+          left[i] = mine[i].count();
+          any[i] = left[i] > 0;
+          pending[i] = false;
+          first_s[i] = first_pv[i] = true;
+        }
+        auto v_bar = [&](int u) {
           const uint32_t pos = base + 2 * u + 1;
-          if (!warp_wait(&kv_full[pos % ST], (pos / ST) & 1, abort_flag, a.status, 63)) return false;
-          if (fresh[t] && n_item[t] > 0 && !warp_wait(&o_empty[t], (n_item[t] - 1) & 1, abort_flag, a.status, 64)) return false;
-          if (!warp_wait(&p_full[t], n_p[t] & 1, abort_flag, a.status, 65)) return false;
-          ++n_p[t];
+          return BandBar{&kv_full[pos % ST], (pos / ST) & 1};
+        };
+        auto k_bar = [&](int u) {
+          const uint32_t pos = base + 2 * u;
+          return BandBar{&kv_full[pos % ST], (pos / ST) & 1};
+        };
+        // O += P V of tile u, whose V is there
+        auto pv = [&](int i, int u, bool last) {
+          const int t = t0 + i;
           tc_fence_after();
-          const uint32_t b_low = desc_mn(ring + (pos % ST) * L::kTile);
-          const bool last = left[t] == 0, first = fresh[t];
           if (one) {
-            mma_apply<32>(tmem + 256 + t * D, tmem + t * 128, b_low, idesc_o, first);
+            const uint32_t b_low = desc_mn(ring + ((base + 2 * u + 1) % ST) * L::kTile);
+            mma_apply<8, kOwn ? 8 : 4, 64>(tmem + 256 + t * D, tmem + (kOwn ? 384 + t * 64 : t * 128), b_low, idesc_o, first_pv[i]);
+            if (kOwn) tc_commit(&pv_done[t]);
             if (last) tc_commit(&o_full[t]);
           }
-          fresh[t] = false;
-          pending[t] = false;
+          ++n_p[i];
+          first_pv[i] = false;
+          pending[i] = false;
+        };
+        auto p_bar = [&](int i) { return BandBar{&p_full[t0 + i], n_p[i] & 1}; };
+        auto o_free = [&](int i) {  // the accumulator, for the first product of an item
+          return !first_pv[i] || n_item[i] == 0 || band_wait(&o_empty[t0 + i], (n_item[i] - 1) & 1, abort_flag, a.status, 64);
+        };
+        // S = Q K^T; the first of an item waits for its queries
+        auto scores = [&](int i, int u) {
+          const int t = t0 + i;
+          if (first_s[i] && !band_wait(&q_full[t], n_item[i] & 1, abort_flag, a.status, 67)) return false;
+          first_s[i] = false;
+          ++n_s[i];
+          tc_fence_after();
+          const bool last = --left[i] == 0;
+          if (one) {
+            mma_scores<D>(tmem + t * 128, desc_k(smem_u32(smem + L::kQ + t * L::kTile)),
+                          desc_k(ring + ((base + 2 * u) % ST) * L::kTile), idesc_s);
+            tc_commit(&s_full[t]);
+            if (last) tc_commit(&q_empty[t]);
+          }
           return true;
+        };
+        auto release = [&](uint32_t pos) {
+          if (one) tc_commit(&kv_empty[pos % ST]);
         };
         for (int u = 0; u < n && ok; ++u) {
           const int j = tile_at(w.all, u);
-          const uint32_t pos = base + 2 * u;
-          if (!warp_wait(&kv_full[pos % ST], (pos / ST) & 1, abort_flag, a.status, 66)) {
-            ok = false;
-            break;
-          }
-          const uint32_t b_low = desc_k(ring + (pos % ST) * L::kTile);
+          if (kOwn) {
+            const bool use = mine[0].uses(j), was = pending[0];
+            // P of the tile before may still be in the making: its product comes after these scores
+            ok = n_s[0] == 0 ? band_wait(k_bar(u).bar, k_bar(u).parity, abort_flag, a.status, 66)
+                             : band_wait_all(abort_flag, a.status, 66, k_bar(u), BandBar{&s_read[t0], (n_s[0] - 1) & 1});
+            if (ok && use) ok = scores(0, u);
+            if (ok) release(base + 2 * u);
+            if (ok && was) {
+              ok = o_free(0) && band_wait_all(abort_flag, a.status, 63, v_bar(u - 1), p_bar(0));
+              if (ok) pv(0, u - 1, left[0] == 0 && !use);
+            }
+            if (ok && u > 0) {  // V of a tile that only the other slot works on: passed on once it is there, not before
+              if (!was) ok = band_wait(v_bar(u - 1).bar, v_bar(u - 1).parity, abort_flag, a.status, 76);
+              if (ok) release(base + 2 * u - 1);
+            }
+            pending[0] = use;
+          } else {
+            bool k_there = false, v_there = u == 0;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (ok && pending[t]) ok = pv(t, u - 1);
-            if (ok && w.t[t].uses(j)) {
-              // the first scores of an item (nothing was multiplied with V since) wait for its queries
-              if (fresh[t] && !pending[t] && !warp_wait(&q_full[t], n_item[t] & 1, abort_flag, a.status, 67)) {
-                ok = false;
-              } else {
-                tc_fence_after();
-                const bool last = --left[t] == 0;
-                if (one) {
-                  mma_scores<D>(tmem + t * 128, desc_k(smem_u32(smem + L::kQ + t * L::kTile)), b_low, idesc_s);
-                  tc_commit(&s_full[t]);
-                  if (last) tc_commit(&q_empty[t]);
-                }
-                pending[t] = true;
+            for (int i = 0; i < kMine; ++i) {
+              const bool use = mine[i].uses(j);
+              if (ok && pending[i]) {
+                ok = o_free(i) && (k_there && v_there ? band_wait(p_bar(i).bar, p_bar(i).parity, abort_flag, a.status, 65)
+                                                      : band_wait_all(abort_flag, a.status, 65, k_bar(u), v_bar(u - 1), p_bar(i)));
+                k_there = v_there = true;
+                if (ok) pv(i, u - 1, left[i] == 0);
               }
+              if (ok && use) {
+                ok = (k_there || band_wait(k_bar(u).bar, k_bar(u).parity, abort_flag, a.status, 66)) && scores(i, u);
+                k_there = true;
+              }
+              pending[i] = use;
+            }
+            ok = ok && (k_there || band_wait(k_bar(u).bar, k_bar(u).parity, abort_flag, a.status, 76)) &&
+                 (v_there || band_wait(v_bar(u - 1).bar, v_bar(u - 1).parity, abort_flag, a.status, 76));
+            if (ok) {
+              release(base + 2 * u);
+              if (u > 0) release(base + 2 * u - 1);
             }
           }
-          if (ok && one) {
-            tc_commit(&kv_empty[pos % ST]);
-            if (u > 0) tc_commit(&kv_empty[(pos - 1) % ST]);
+        }
+        bool v_there = false;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          if (ok && pending[i]) {
+            ok = o_free(i) && band_wait_all(abort_flag, a.status, 65, v_bar(n - 1), p_bar(i));
+            v_there = true;
+            if (ok) pv(i, n - 1, true);
           }
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && pending[t]) ok = pv(t, n - 1);
-        if (ok && n > 0 && one) tc_commit(&kv_empty[(base + 2 * n - 1) % ST]);
+        if (ok && n > 0) {
+          if (!v_there) ok = band_wait(v_bar(n - 1).bar, v_bar(n - 1).parity, abort_flag, a.status, 76);
+          if (ok) release(base + 2 * n - 1);
+        }
         base += 2 * n;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) n_item[t] += any[t];
+        for (int i = 0; i < kMine; ++i) n_item[i] += any[i];
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    NMB_BAND_MORE_REGISTERS;
     // ------------------------------------------------- softmax + epilogue --
-    const int t = warp >> 2, quad = warp & 3;
+    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
     const int r = quad * 32 + lane;  // row in the tile == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t t_s = t_row + t * 128, t_o = t_row + 256 + t * D;
+    const uint32_t t_s = t_row + t * 128 + half * 64, t_o = t_row + 256 + t * D + half * (D / 2);
+    const uint32_t t_p = kOwn ? t_row + 384 + t * 64 + half * 32 : t_s;
     const float sl2 = a.scale * kBandLog2e;
     float* lut = luts + t * entries;
-    int n_s = 0, n_item = 0;
-    uint32_t sync_phase = 0;
+    float* xch = reinterpret_cast<float*>(smem + L::kXch) + t * 256 + r;
+    int n_s = 0, n_item = 0, parity = 0;
     bool ok = true;
-    for (int round = 0; ok; ++round) {
+    // the other thread's value of this row
+    auto other = [&](float mine) {
+      float* x = xch + parity * 512;
+      parity ^= 1;
+      x[half * 128] = mine;
+      named_sync(1 + t * 4 + quad, 64);
+      return x[(half ^ 1) * 128];
+    };
+    for (int round = 0;; ++round) {
       const int item = item_of_round(round);
       if (round * static_cast<int>(gridDim.x) >= p.n_items) break;
       if (item >= p.n_items) continue;
       const FwdItem w = fwd_item(p, item);
-      const int q0 = w.q0[t], h = w.h[t];
-      const KeyTiles mine = w.t[t];
+      const int q0 = t == 0 ? w.q0[0] : w.q0[1], h = t == 0 ? w.h[0] : w.h[1];
+      const KeyTiles mine = t == 0 ? w.t[0] : w.t[1];
       if (q0 < 0) continue;
       const int row = q0 + r, pos = a.q_pos0 + row;
       const int pmin = a.q_pos0 + q0, pmax = pmin + 127;
       float far_bias = 0.f;
       if (a.table != nullptr) {
-        ok = group_sync(&sync_bar[t], sync_phase, abort_flag, a.status, 70);  // everyone has left the item before
-        build_lut(a, h, p.t_last, map, lut, r, 128);
-        ok = ok && group_sync(&sync_bar[t], sync_phase, abort_flag, a.status, 71);
-        if (!ok) break;
+        named_sync(9 + t, 256);  // everyone has left the item before
+        build_lut(a, h, p.t_last, map, lut, threadIdx.x & 255, 256);
+        named_sync(9 + t, 256);
         far_bias = lut[entries - 1];
       }
       const int n = mine.count();
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // l: of this thread's keys
       for (int u = 0; u < n; ++u) {
         const int kv0 = tile_at(mine, u) * 128;
-        if (!warp_wait(&s_full[t], n_s & 1, abort_flag, a.status, 68)) {
-          ok = false;
-          break;
-        }
+        NMB_BAND_WAIT(&s_full[t], n_s & 1, 68);
         ++n_s;
         tc_fence_after();
-        uint32_t s[4][32];
+        uint32_t s[2][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, s[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32(t_s + c * 32, s[c]);
         tmem_ld_wait();
+        if (kOwn) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_read[t]);
+        }
         float mul = sl2, add = far_bias;
         // Biases that differ inside the tile, or that are too large to be added to the maximum instead of to the scores.
-        if (a.table != nullptr && (pmin - (kv0 + 127) < p.t_last || fabsf(far_bias) > 1e30f)) {
-          const float* at = lut + kLutFront + min(pos - kv0, p.t_last + kLutBack - 1);
+        const bool added = a.table != nullptr && (pmin - (kv0 + 127) < p.t_last || fabsf(far_bias) > 1e30f);
+        if (added) {
+          const float* at = lut + kLutFront + min(pos - kv0, p.t_last + kLutBack - 1) - half * 64;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(fmaf(__uint_as_float(s[c][k]), sl2, at[-(c * 32 + k)]));
           mul = 1.f;
           add = 0.f;
         }
+        // What this warp's rows see of each chunk of 32 keys: all (1), none (2), or some (0).
         const bool whole = kv0 + 127 <= pmin && kv0 + 127 < a.Skv && (kv0 > pmax - a.window || kv0 + 127 < a.sinks);
+        uint32_t part[2] = {1, 1};
         if (!whole) {
-          const int hi = min(pos, a.Skv - 1) - kv0 + 1, lo = pos - a.window + 1 - kv0, sk = a.sinks - kv0;
+          const int k0 = kv0 + half * 64;
+          const int hi = min(pos, a.Skv - 1) - k0 + 1, lo = pos - a.window + 1 - k0, sk = a.sinks - k0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             const uint32_t see = low_bits(hi - c * 32) & (~low_bits(lo - c * 32) | low_bits(sk - c * 32));
+            part[c] = __all_sync(0xffffffffu, see == ~0u) ? 1u : __all_sync(0xffffffffu, see == 0u) ? 2u : 0u;
+            if (part[c] == 0) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!((see >> k) & 1u)) s[c][k] = 0xff800000u;
+              for (int k = 0; k < 32; ++k)
+                if (!((see >> k) & 1u)) s[c][k] = 0xff800000u;
+            }
           }
         }
-        float mx[4];
+        float mx[2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = __uint_as_float(s[c][0]);
+        for (int c = 0; c < 2; ++c) {
+          mx[c] = -INFINITY;
+          if (part[c] != 2) {
+            float m0 = __uint_as_float(s[c][0]), m1 = __uint_as_float(s[c][1]);
 #pragma unroll
-          for (int k = 1; k < 32; ++k) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][k]));
+            for (int k = 2; k < 30; k += 4) {
+              m0 = max3(m0, __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+              m1 = max3(m1, __uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3]));
+            }
+            mx[c] = max3(fmaxf(m0, m1), __uint_as_float(s[c][30]), __uint_as_float(s[c][31]));
+          }
         }
-        const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), mul, add);
+        float top = fmaf(fmaxf(mx[0], mx[1]), mul, add);
+        top = fmaxf(top, other(top));
         // The maximum that weights are relative to moves only when it grew by more than 2^8: most tiles need no pass over O,
         // and the division by the sum at the end makes the result exact.
         const float m_new = top > m + 8.f ? top : m;
         const float alpha = m_new == m ? 1.f : ex2(m - m_new);  // m == -inf: 0
         const float shift = add - (m_new == -INFINITY ? 0.f : m_new);
-        float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float p0 = ex2(fmaf(__uint_as_float(s[c][2 * k]), mul, shift));
-            const float p1 = ex2(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, shift));
-            sum0 += p0;
-            sum1 += p1;
-            pk[k] = pack_bf16x2(p0, p1);
-          }
-          tmem_st_32x16(t_s + c * 16, pk);
-        }
-        // the scores are complete, so is the product of the tile before: O may be rescaled
+        // The product of the tile before is done: with shared columns the scores came after it.
+        if (kOwn && n_s > 1) NMB_BAND_WAIT(&pv_done[t], n_s & 1, 73);
         if (u > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(t_o + c * 32, o);
+            uint32_t o[16];
+            tmem_ld_32x16(t_o + c * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st_32x32(t_o + c * 32, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st_32x16(t_o + c * 16, o);
           }
         }
-        l = l * alpha + (sum0 + sum1);
-        m = m_new;
+        const uint64_t mul_2 = pack2(mul, mul), shift_2 = pack2(shift, shift);
+        uint64_t sum = pack2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+          if (part[c] == 2) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) pk[k] = 0;
+          } else if (part[c] == 1 && !added) {
+            weights32<true>(s[c], mul_2, shift_2, sum, pk);
+          } else {
+            weights32<false>(s[c], mul_2, shift_2, sum, pk);
+          }
+          tmem_st_32x16(t_p + c * 16, pk);
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
+        float sum0, sum1;
+        unpack2(sum, sum0, sum1);
+        l = l * alpha + (sum0 + sum1);
+        m = m_new;
       }
-      if (!ok) break;
-      const long long stat = (static_cast<long long>(w.b) * a.Hq + h) * a.Sq + row;
-      __nv_bfloat16* out = band_row(a.o, a.o_st, w.b, row, h);
       if (n > 0) {
-        if (!warp_wait(&o_full[t], n_item & 1, abort_flag, a.status, 69)) {
-          ok = false;
-          break;
-        }
+        l += other(l);
+        NMB_BAND_WAIT(&o_full[t], n_item & 1, 69);
         ++n_item;
         tc_fence_after();
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
+      __nv_bfloat16* out = band_row(a.o, a.o_st, w.b, row, h) + half * (D / 2);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
+        uint32_t o[16];
         if (n > 0) {
-          tmem_ld_32x32(t_o + c * 32, o);
+          tmem_ld_32x16(t_o + c * 16, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0;
+          for (int k = 0; k < 16; ++k) o[k] = 0;
         }
-        if (row < a.Sq) store_bf16_32(out + c * 32, o, inv);
+        if (row < a.Sq) store_bf16_16(out + c * 16, o, inv);
       }
       if (n > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_empty[t]);
       }
-      if (row < a.Sq) {
+      if (half == 0 && row < a.Sq) {
+        const long long stat = (static_cast<long long>(w.b) * a.Hq + h) * a.Sq + row;
         a.m[stat] = l > 0.f ? m : INFINITY;  // a row that sees nothing: 2^(x - m) is 0 in the backward pass
         a.l[stat] = l > 0.f ? log2f(l) : 0.f;
       }
@@ -628,7 +880,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) band_fwd_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -645,7 +897,7 @@ static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStr
 template <int D>
 static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
   const int lut = p.a.table == nullptr ? 0 : lut_bytes(p.t_last, 2);
-  return launch_pdl(band_fwd_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kFwdThreads), BandFwdSmem<D>::kLut + lut, s, p);
+  return launch_pdl(band_fwd_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
 }
 
 // --------------------------------------------------------------- backward --
@@ -654,29 +906,33 @@ static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
 //
 // Column statistics passed from the first to the second, per (batch, query head, query tile): 128 floats each of
 //   c = (far bias - m) - l,  D,  m,  l        (rows behind the last: c = -inf, so that their weights are 0)
-constexpr int kBwdBandThreads = 384;
 constexpr int kStatBlock = 512;  // floats
 
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-// 16 consecutive values of a row as bf16
-__device__ __forceinline__ void store_bf16_16(__nv_bfloat16* dst, const uint32_t (&r)[16], float mul) {
-  uint32_t w[8];
+// 2^(s * mul + shift) of 32 scores in place
+template <bool kMix>
+__device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, uint64_t shift) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(__uint_as_float(r[2 * k]) * mul, __uint_as_float(r[2 * k + 1]) * mul);
-  st_global_32(dst, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+  for (int k = 0; k < 16; ++k) {
+    float p0, p1;
+    exp2_pair<kMix>(k, fma2(pack2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), mul, shift), p0, p1);
+    s[2 * k] = __float_as_uint(p0);
+    s[2 * k + 1] = __float_as_uint(p1);
+  }
 }
-__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// the same with a shift per column
+template <bool kMix>
+__device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, const float* shift) {
+#pragma unroll
+  for (int k = 0; k < 16; k += 2) {
+    const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(shift + 2 * k);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float p0, p1;
+      exp2_pair<kMix>(k + i, fma2(pack2(__uint_as_float(s[2 * (k + i)]), __uint_as_float(s[2 * (k + i) + 1])), mul, i ? c.y : c.x), p0, p1);
+      s[2 * (k + i)] = __float_as_uint(p0);
+      s[2 * (k + i) + 1] = __float_as_uint(p1);
+    }
+  }
 }
 
 struct BandBwdParams {
@@ -693,7 +949,7 @@ struct BandBwdParams {
 };
 
 // ---- dQ, D, and the table's gradient ----
-// A CTA works on one query tile: S = Q K^T and dP = dO V^T land in tensor memory, eight warps (two threads a row, 64 columns
+// A CTA works on one query tile: S = Q K^T and dP = dO V^T land in tensor memory, sixteen warps (four threads a row, 32 columns
 // each) turn them into dS, which goes back as the A operand of dQ += dS K.  S and dP of the next tile are computed while
 // dS of this one is.  TMEM: S 0, dP 128, dQ 256, dS (two buffers) from 384.
 //
@@ -706,15 +962,20 @@ struct BandDqSmem {
   static constexpr int kSlabs = (D + 63) / 64;
   static constexpr int kTile = kSlabs * 16384;
   static constexpr int kQStages = D == 64 ? 2 : 1;
-  static constexpr int kStages = D == 64 ? 8 : 4;  // K and V tiles in turn
+  // K stays until dQ += dS K, V only until dP: where four tiles is all there is room for, three are for K (a ring of two
+  // pairs left the loads of K exposed: 1640 of 4020 clocks a tile were spent waiting at d = 128)
+  static constexpr int kStagesK = D == 64 ? 4 : 3, kStagesV = D == 64 ? 4 : 1;
+  static constexpr int kStages = kStagesK + kStagesV;
   static constexpr int kQ = 0;                     // Q, dO per stage
-  static constexpr int kRing = 2 * kQStages * kTile;
+  static constexpr int kRing = 2 * kQStages * kTile;  // the stages of K, then those of V
   static constexpr int kBar = kRing + kStages * kTile;
-  static constexpr int kNumBars = 2 * kStages + 2 * kQStages + 6;
-  static constexpr int kXch = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [2][2][128]
-  static constexpr int kLut = kXch + 2048;                                     // float [entries], the map
-  // behind them, where the table's gradient is wanted: float bins[8][128], diagonals[8][96]
-  static constexpr int kBins = 8 * (kMaxBuckets + 96) * 4;
+  static constexpr int kNumBars = 2 * kStages + 2 * kQStages + 8;
+  static constexpr int kXch = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [2][4][128]
+  static constexpr int kLut = kXch + 4096;                                     // float [entries], the map
+  // behind them, where the table's gradient is wanted: float bins[16][128], diagonals[16][64]
+  static constexpr int kBins = kComputeWarps * (kMaxBuckets + 64) * 4;
+  // columns of a row that one of its four threads reads and writes; three do at D = 96
+  static constexpr int kCols = D == 96 ? 32 : D / 4;
 };
 
 // The query tile of an item, longest first.
@@ -735,21 +996,22 @@ __device__ __forceinline__ DqItem dq_item(const BandBwdParams& p, int item) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const __grid_constant__ BandBwdParams p) {
+__global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __grid_constant__ BandBwdParams p) {
   using L = BandDqSmem<D>;
-  constexpr int NS = L::kSlabs, ST = L::kStages, QS = L::kQStages;
+  constexpr int NS = L::kSlabs, ST = L::kStages, SK = L::kStagesK, SV = L::kStagesV, QS = L::kQStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* kv_full = bars;                // [ST]
-  uint64_t* kv_empty = bars + ST;          // [ST]
+  uint64_t* kv_full = bars;                // [SK + SV]
+  uint64_t* kv_empty = bars + ST;          // [SK + SV]
   uint64_t* q_full = bars + 2 * ST;        // [QS]
-  uint64_t* q_empty = q_full + QS;         // [QS] last product issued + 8 warps that read dO
+  uint64_t* q_empty = q_full + QS;         // [QS] last product issued + the warps that read dO
   uint64_t* sdp_full = q_empty + QS;
   uint64_t* sdp_read = sdp_full + 1;
-  uint64_t* ds_full = sdp_full + 2;
-  uint64_t* dq_full = sdp_full + 3;
-  uint64_t* dq_empty = sdp_full + 4;
-  uint64_t* sync_bar = sdp_full + 5;
+  uint64_t* dq_full = sdp_full + 2;
+  uint64_t* dq_empty = sdp_full + 3;
+  // one for even and one for odd steps, as the buffers of dS: with one, a step could be over twice before it was looked at
+  uint64_t* ds_full = sdp_full + 4;      // [2]
+  uint64_t* step_done = sdp_full + 6;    // [2] dQ += dS K of a step
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const BandArgs& a = p.a;
@@ -771,36 +1033,43 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
     }
     for (int s = 0; s < QS; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 9);
+      mbar_init(&q_empty[s], 1 + kComputeWarps);
     }
     mbar_init(sdp_full, 1);
-    mbar_init(sdp_read, 8);
-    mbar_init(ds_full, 8);
+    mbar_init(sdp_read, kComputeWarps);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ds_full[s], kComputeWarps);
+      mbar_init(&step_done[s], 1);
+    }
     mbar_init(dq_full, 1);
-    mbar_init(dq_empty, 8);
-    mbar_init(sync_bar, 8);
+    mbar_init(dq_empty, kComputeWarps);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   if (a.table != nullptr) {
-    build_bucket_map(a, p.t_last, map, threadIdx.x, kBwdBandThreads);
+    build_bucket_map(a, p.t_last, map, threadIdx.x, kBandThreads);
     if (a.dtable != nullptr)
-      for (int n = threadIdx.x; n < 8 * kMaxBuckets; n += kBwdBandThreads) bins[n] = 0.f;
+      for (int n = threadIdx.x; n < kComputeWarps * kMaxBuckets; n += kBandThreads) bins[n] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // All 512 columns were allocated, so they begin at 0; said as a constant the addresses need no moves to uniform registers.
+  constexpr uint32_t tmem = 0;
+  if (threadIdx.x == 0 && *tmem_slot != 0) {
+    report_status(a.status, kBadArgument, 75);
+    *abort_flag = 1;
+  }
   pdl_enter();
   const int rounds = (p.n_items + gridDim.x - 1) / gridDim.x;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8 && lane == 0) {
+  if (warp >= kComputeWarps) {
+    NMB_BAND_FEW_REGISTERS;
+    if (warp == kLoadWarp && lane == 0) {
       // ---------------------------------------------------------- producer --
       tma_prefetch_desc(&p.q_map);
       tma_prefetch_desc(&p.do_map);
@@ -816,7 +1085,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
         if (n == 0) continue;
         const int qs = n_item % QS, use = n_item / QS;
         ++n_item;
-        if (use > 0 && !mbar_wait(&q_empty[qs], (use - 1) & 1, abort_flag, a.status, 81)) break;
+        if (use > 0 && !band_wait(&q_empty[qs], (use - 1) & 1, abort_flag, a.status, 81)) break;
         mbar_expect_tx(&q_full[qs], 2 * L::kTile);
 #pragma unroll
         for (int c = 0; c < NS; ++c) {
@@ -824,42 +1093,26 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
           tma_load_4d(dst, &p.q_map, &q_full[qs], c * 64, w.q0, w.h, w.b);
           tma_load_4d(dst + L::kTile, &p.do_map, &q_full[qs], c * 64, w.q0, w.h, w.b);
         }
-        for (int u = 0; u < 2 * n; ++u, ++pos) {
-          const int st = pos % ST, kuse = pos / ST, j = tile_at(w.t, u >> 1);
-          if (kuse > 0 && !mbar_wait(&kv_empty[st], (kuse - 1) & 1, abort_flag, a.status, 82)) {
-            ok = false;
-            break;
-          }
+        auto load = [&](const CUtensorMap* m, int st, int use, int j) {
+          if (use > 0 && !band_wait(&kv_empty[st], (use - 1) & 1, abort_flag, a.status, 82)) return false;
           mbar_expect_tx(&kv_full[st], L::kTile);
 #pragma unroll
           for (int c = 0; c < NS; ++c)
-            tma_load_4d(smem + L::kRing + st * L::kTile + c * 16384, (u & 1) ? &p.v_map : &p.k_map, &kv_full[st], c * 64,
-                        j * 128, w.hk, w.b);
+            tma_load_4d(smem + L::kRing + st * L::kTile + c * 16384, m, &kv_full[st], c * 64, j * 128, w.hk, w.b);
+          return true;
+        };
+        for (int u = 0; u < n && ok; ++u, ++pos) {
+          const int j = tile_at(w.t, u);
+          ok = load(&p.k_map, pos % SK, pos / SK, j) && load(&p.v_map, SK + pos % SV, pos / SV, j);
         }
       }
-    } else if (warp == 9) {
-      // -------------------------------------------------------- MMA issuer --
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------- MMA issuer: S and dP --
       constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
-      constexpr uint32_t idesc_dq = make_idesc_bf16(128, D, false, true);
       const uint32_t ring = smem_u32(smem + L::kRing);
       const bool one = elect_one();
       uint32_t step = 0, n_item = 0;  // tiles and items begun
-      bool prev_first = false, prev_last = false;
-      uint32_t prev_item = 0;
       bool ok = true;
-      // dQ += dS K of step s
-      auto issue_dq = [&](uint32_t s, bool first, bool last, uint32_t item_no) {
-        if (first && item_no > 0 && !warp_wait(dq_empty, (item_no - 1) & 1, abort_flag, a.status, 83)) return false;
-        if (!warp_wait(ds_full, s & 1, abort_flag, a.status, 84)) return false;
-        tc_fence_after();
-        const uint32_t st = 2 * s % ST;
-        if (one) {
-          mma_apply<32>(tmem + kDq, tmem + kDs + (s & 1) * 64, desc_mn(ring + st * L::kTile), idesc_dq, first);
-          tc_commit(&kv_empty[st]);
-          if (last) tc_commit(dq_full);
-        }
-        return true;
-      };
       for (int round = 0; round < rounds && ok; ++round) {
         const int item = item_of_round(round);
         if (item >= p.n_items) continue;
@@ -869,46 +1122,80 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
         const uint32_t qs = n_item % QS;
         const uint32_t q_low = desc_k(smem_u32(smem + L::kQ + 2 * qs * L::kTile));
         for (int u = 0; u < n; ++u, ++step) {
-          const uint32_t pk = 2 * step, pv = pk + 1;
-          ok = (u > 0 || warp_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 85)) &&
-               warp_wait(&kv_full[pk % ST], (pk / ST) & 1, abort_flag, a.status, 86) &&
-               warp_wait(&kv_full[pv % ST], (pv / ST) & 1, abort_flag, a.status, 87) &&
-               (step == 0 || warp_wait(sdp_read, (step - 1) & 1, abort_flag, a.status, 88));
+          const uint32_t sk = step % SK, sv = SK + step % SV;
+          // the buffer of dS that this step's scores will fill was last read two steps ago; done before they are is done
+          // before anyone writes to it
+          ok = (u > 0 || band_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 85)) &&
+               band_wait(&kv_full[sk], (step / SK) & 1, abort_flag, a.status, 86) &&
+               (step < 2 || band_wait(&step_done[step & 1], ((step - 2) >> 1) & 1, abort_flag, a.status, 83)) &&
+               (step == 0 || band_wait(sdp_read, (step - 1) & 1, abort_flag, a.status, 88));
           if (!ok) break;
           tc_fence_after();
+          if (one) mma_scores<D>(tmem, q_low, desc_k(ring + sk * L::kTile), idesc_s);
+          ok = band_wait(&kv_full[sv], (step / SV) & 1, abort_flag, a.status, 87);
+          if (!ok) break;
           if (one) {
-            mma_scores<D>(tmem, q_low, desc_k(ring + (pk % ST) * L::kTile), idesc_s);
-            mma_scores<D>(tmem + kDp, q_low + (L::kTile >> 4), desc_k(ring + (pv % ST) * L::kTile), idesc_s);
+            mma_scores<D>(tmem + kDp, q_low + (L::kTile >> 4), desc_k(ring + sv * L::kTile), idesc_s);
             tc_commit(sdp_full);
-            tc_commit(&kv_empty[pv % ST]);
+            tc_commit(&kv_empty[sv]);
             if (u == n - 1) tc_commit(&q_empty[qs]);
           }
-          if (step > 0) ok = issue_dq(step - 1, prev_first, prev_last, prev_item);
-          if (!ok) break;
-          prev_first = u == 0;
-          prev_last = u == n - 1;
-          prev_item = n_item;
         }
         ++n_item;
       }
-      if (ok && step > 0) issue_dq(step - 1, prev_first, prev_last, prev_item);
+    } else if (warp == kMmaWarp + 1) {
+      // ----------------------------------------------------- MMA issuer: dQ --
+      constexpr uint32_t idesc_dq = make_idesc_bf16(128, D, false, true);
+      const uint32_t ring = smem_u32(smem + L::kRing);
+      const bool one = elect_one();
+      uint32_t step = 0, n_item = 0;
+      bool ok = true;
+      for (int round = 0; round < rounds && ok; ++round) {
+        const int item = item_of_round(round);
+        if (item >= p.n_items) continue;
+        const int n = dq_item(p, item).t.count();
+        if (n == 0) continue;
+        for (int u = 0; u < n; ++u, ++step) {
+          const uint32_t sk = step % SK;
+          ok = band_wait(&kv_full[sk], (step / SK) & 1, abort_flag, a.status, 93) &&
+               (u > 0 || n_item == 0 || band_wait(dq_empty, (n_item - 1) & 1, abort_flag, a.status, 94)) &&
+               band_wait(&ds_full[step & 1], (step >> 1) & 1, abort_flag, a.status, 84);
+          if (!ok) break;
+          tc_fence_after();
+          if (one) {
+            mma_apply<8, 8, 0>(tmem + kDq, tmem + kDs + (step & 1) * 64, desc_mn(ring + sk * L::kTile), idesc_dq, u == 0);
+            tc_commit(&step_done[step & 1]);
+            tc_commit(&kv_empty[sk]);
+            if (u == n - 1) tc_commit(dq_full);
+          }
+        }
+        ++n_item;
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    NMB_BAND_MORE_REGISTERS;
     // ------------------------------------------------------------ compute --
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, quarter = warp >> 2;
     const int r = quad * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const bool has_cols = quarter * L::kCols < D;
     float* xch = reinterpret_cast<float*>(smem + L::kXch);
     float* my_bins = bins + warp * kMaxBuckets;
-    float* diag = bins + 8 * kMaxBuckets + warp * 96;
+    float* diag = bins + kComputeWarps * kMaxBuckets + warp * 64;
     const float sl2 = a.scale * kBandLog2e;
     const bool want_table = a.dtable != nullptr;
     int step = 0, n_item = 0, parity = 0;
-    uint32_t sync_phase = 0;
-    auto together = [&]() { return group_sync(sync_bar, sync_phase, abort_flag, a.status, 92); };
+    auto together = [&]() { named_sync(1, kComputeWarps * 32); };
+    // the sum of a row's four values
+    auto row_sum = [&](float mine) {
+      float* x = xch + parity * 512 + r;
+      parity ^= 1;
+      x[quarter * 128] = mine;
+      together();
+      return (x[0] + x[128]) + (x[256] + x[384]);
+    };
     bool ok = true;
-    for (int round = 0; round < rounds && ok; ++round) {
+    for (int round = 0; round < rounds; ++round) {
       const int item = item_of_round(round);
       if (item >= p.n_items) continue;
       const DqItem w = dq_item(p, item);
@@ -920,42 +1207,43 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
       const float l = valid ? a.l[at_row] : 0.f;
       float far_bias = 0.f;
       if (a.table != nullptr) {
-        if (!together()) break;  // everyone has left the item before
-        build_lut(a, w.h, p.t_last, map, lut, threadIdx.x, 256);
+        together();  // everyone has left the item before
+        build_lut(a, w.h, p.t_last, map, lut, threadIdx.x, kComputeWarps * 32);
       }
-      // D: half a row of O and dO per thread
+      // D: a quarter of a row of O and dO per thread
       float dsum = 0.f;
       if (n > 0) {
-        constexpr int kChunks = D / 16;  // 16-byte chunks of half a row
+        constexpr int kChunks = L::kCols / 8;  // of 16 bytes
         uint4 o[kChunks];
-        const uint4* src = reinterpret_cast<const uint4*>(band_row(a.o, a.o_st, w.b, valid ? row : w.q0, w.h)) + half * kChunks;
+        if (has_cols) {
+          const uint4* src = reinterpret_cast<const uint4*>(band_row(a.o, a.o_st, w.b, valid ? row : w.q0, w.h)) + quarter * kChunks;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) o[c] = src[c];
+          for (int c = 0; c < kChunks; ++c) o[c] = src[c];
+        }
         const int qs = n_item % QS;
-        if (!warp_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 89)) break;
-        const uint8_t* sdo = smem + L::kQ + (2 * qs + 1) * L::kTile;
+        NMB_BAND_WAIT(&q_full[qs], (n_item / QS) & 1, 89);
+        if (has_cols) {
+          const uint8_t* sdo = smem + L::kQ + (2 * qs + 1) * L::kTile;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int ch = half * kChunks + c;
-          const uint4 g = *reinterpret_cast<const uint4*>(sdo + (ch >> 3) * 16384 + swz128_offset(r, ch & 7));
-          const uint32_t ow[4] = {o[c].x, o[c].y, o[c].z, o[c].w}, gw[4] = {g.x, g.y, g.z, g.w};
+          for (int c = 0; c < kChunks; ++c) {
+            const int ch = quarter * kChunks + c;
+            const uint4 g = *reinterpret_cast<const uint4*>(sdo + (ch >> 3) * 16384 + swz128_offset(r, ch & 7));
+            const uint32_t ow[4] = {o[c].x, o[c].y, o[c].z, o[c].w}, gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 x = unpack_bf16x2(ow[k]), y = unpack_bf16x2(gw[k]);
-            dsum = fmaf(x.x, y.x, fmaf(x.y, y.y, dsum));
+            for (int k = 0; k < 4; ++k) {
+              const float2 x = unpack_bf16x2(ow[k]), y = unpack_bf16x2(gw[k]);
+              dsum = fmaf(x.x, y.x, fmaf(x.y, y.y, dsum));
+            }
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[qs]);
       }
-      float* mine = xch + parity * 256;
-      parity ^= 1;
-      mine[half * 128 + r] = dsum;
-      if (!together()) break;
-      const float delta = valid ? mine[r] + mine[128 + r] : 0.f;
+      dsum = row_sum(dsum);
+      const float delta = valid ? dsum : 0.f;
       if (a.table != nullptr) far_bias = lut[entries - 1];
       const float c_far = (far_bias - m) - l;
-      if (half == 0) {
+      if (quarter == 0) {
         float* st = p.stat + ((static_cast<long long>(w.b) * a.Hq + w.h) * p.n_qt + w.q0 / 128) * kStatBlock + r;
         st[0] = c_far;
         st[128] = delta;
@@ -964,18 +1252,12 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
       }
       float ds_all = 0.f, ds_far = 0.f, p_far = 0.f;
       for (int u = 0; u < n; ++u, ++step) {
-        const int kv0 = tile_at(w.t, u) * 128;
-        if (!warp_wait(sdp_full, step & 1, abort_flag, a.status, 90)) {
-          ok = false;
-          break;
-        }
+        const int kv0 = tile_at(w.t, u) * 128, k0 = kv0 + quarter * 32;
+        NMB_BAND_WAIT(sdp_full, step & 1, 90);
         tc_fence_after();
-        uint32_t s[2][32], dp[2][32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tmem_ld_32x32(t_row + half * 64 + c * 32, s[c]);
-          tmem_ld_32x32(t_row + kDp + half * 64 + c * 32, dp[c]);
-        }
+        uint32_t s[32], dp[32];
+        tmem_ld_32x32(t_row + quarter * 32, s);
+        tmem_ld_32x32(t_row + kDp + quarter * 32, dp);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -984,80 +1266,70 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
         const bool added = near || (a.table != nullptr && fabsf(far_bias) > 1e30f);
         const bool whole = kv0 + 127 <= pmin && kv0 + 127 < a.Skv && (pmin + 127 - kv0 < a.window || kv0 + 127 < a.sinks);
         // weights, in place of the scores
-        if (!added) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(ex2(fmaf(__uint_as_float(s[c][k]), sl2, c_far)));
+        if (whole && !added && w.q0 + 128 <= a.Sq) {  // every row sees finite scores: no weight has to come out as 0
+          exps32<true>(s, pack2(sl2, sl2), pack2(c_far, c_far));
+        } else if (!added) {
+          exps32<false>(s, pack2(sl2, sl2), pack2(c_far, c_far));
         } else {
-          const float* at = lut + kLutFront + min(pos - kv0, p.t_last + kLutBack - 1) - half * 64;
+          const float* at = lut + kLutFront + min(pos - kv0, p.t_last + kLutBack - 1) - quarter * 32;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              s[c][k] = __float_as_uint(ex2((fmaf(__uint_as_float(s[c][k]), sl2, at[-(c * 32 + k)]) - m) - l));
+          for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(ex2((fmaf(__uint_as_float(s[k]), sl2, at[-k]) - m) - l));
         }
         if (!whole) {
-          const int hi = min(pos, a.Skv - 1) - kv0 + 1, lo = pos - a.window + 1 - kv0, sk = a.sinks - kv0;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int c0 = half * 64 + c * 32;
-            const uint32_t see = low_bits(hi - c0) & (~low_bits(lo - c0) | low_bits(sk - c0));
+          const uint32_t see = low_bits(min(pos, a.Skv - 1) - k0 + 1) & (~low_bits(pos - a.window + 1 - k0) | low_bits(a.sinks - k0));
+          if (!__all_sync(0xffffffffu, see == ~0u)) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (!((see >> k) & 1u)) s[c][k] = 0;
+              if (!((see >> k) & 1u)) s[k] = 0;
           }
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        {
           uint32_t pk[16];
+          const uint64_t minus = pack2(-delta, -delta);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) dp[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * (__uint_as_float(dp[c][k]) - delta));
-#pragma unroll
-          for (int k = 0; k < 16; ++k) pk[k] = pack_bf16x2(__uint_as_float(dp[c][2 * k]), __uint_as_float(dp[c][2 * k + 1]));
-          tmem_st_32x16(t_row + kDs + (step & 1) * 64 + half * 32 + c * 16, pk);
+          for (int k = 0; k < 16; ++k) {
+            float d0, d1;
+            unpack2(mul2(pack2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])),
+                         add2(pack2(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1])), minus)), d0, d1);
+            dp[2 * k] = __float_as_uint(d0);
+            dp[2 * k + 1] = __float_as_uint(d1);
+            pk[k] = pack_bf16x2(d0, d1);
+          }
+          tmem_st_32x16(t_row + kDs + (step & 1) * 64 + quarter * 16, pk);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
+        if (lane == 0) mbar_arrive(&ds_full[step & 1]);
         if (want_table) {
           float sum = 0.f;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; ++k) sum += __uint_as_float(dp[c][k]);
+          for (int k = 0; k < 32; ++k) sum += __uint_as_float(dp[k]);
           ds_all += sum;
-          const int far_from = pos - kv0 - p.t_last - half * 64;  // columns up to this one belong to the last bucket
           if (!near) {
             ds_far += sum;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) p_far += __uint_as_float(s[c][k]);
+            for (int k = 0; k < 32; ++k) p_far += __uint_as_float(s[k]);
           } else {
+            const int far_to = pos - k0 - p.t_last;  // columns up to this one belong to the last bucket
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) p_far += c * 32 + k <= far_from ? __uint_as_float(s[c][k]) : 0.f;
+            for (int k = 0; k < 32; ++k) p_far += k <= far_to ? __uint_as_float(s[k]) : 0.f;
             // diagonal e holds distance base + e; lane 31 completes one of them per column, the others stay behind at the end
-            const int base = pmin + quad * 32 - kv0 - half * 64 - 63;
+            const int base = pmin + quad * 32 - k0 - 31;
             float run = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const float from = __shfl_up_sync(0xffffffffu, run, 1);
-                run = (lane == 0 ? 0.f : from) + __uint_as_float(dp[c][k]);
-                if (lane == 31) diag[31 + 63 - (c * 32 + k)] = run;
-              }
+            for (int k = 0; k < 32; ++k) {
+              const float from = __shfl_up_sync(0xffffffffu, run, 1);
+              run = (lane == 0 ? 0.f : from) + __uint_as_float(dp[k]);
+              if (lane == 31) diag[31 + 31 - k] = run;
+            }
             if (lane < 31) diag[lane] = run;
             __syncwarp();
 #pragma unroll
-            for (int e0 = 0; e0 < 96; e0 += 32) {
+            for (int e0 = 0; e0 < 64; e0 += 32) {
               const int e = e0 + lane;
-              float v = e < 95 ? diag[e] : 0.f;
-              const int bucket = map[kLutFront + base + min(e, 94)];
+              float v = e < 63 ? diag[e] : 0.f;
+              const int bucket = map[kLutFront + base + min(e, 62)];
               // sums over runs of equal buckets; the last lane of a run adds its
 #pragma unroll
               for (int o = 1; o < 32; o <<= 1) {
@@ -1072,24 +1344,25 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
           }
         }
       }
-      if (!ok) break;
-      __nv_bfloat16* out = band_row(a.dq, a.dq_st, w.b, row, w.h) + half * (D / 2);
       if (n > 0) {
-        if (!warp_wait(dq_full, n_item & 1, abort_flag, a.status, 91)) break;
+        NMB_BAND_WAIT(dq_full, n_item & 1, 91);
         ++n_item;
         tc_fence_after();
       }
+      if (has_cols) {
+        __nv_bfloat16* out = band_row(a.dq, a.dq_st, w.b, row, w.h) + quarter * L::kCols;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[16];
-        if (n > 0) {
-          tmem_ld_32x16(t_row + kDq + half * (D / 2) + c * 16, v);
-          tmem_ld_wait();
-        } else {
+        for (int c = 0; c < L::kCols / 16; ++c) {
+          uint32_t v[16];
+          if (n > 0) {
+            tmem_ld_32x16(t_row + kDq + quarter * L::kCols + c * 16, v);
+            tmem_ld_wait();
+          } else {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = 0;
+            for (int k = 0; k < 16; ++k) v[k] = 0;
+          }
+          if (valid) store_bf16_16(out + c * 16, v, a.scale);
         }
-        if (valid) store_bf16_16(out + c * 16, v, a.scale);
       }
       if (n > 0) {
         tc_fence_before();
@@ -1097,25 +1370,21 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
         if (lane == 0) mbar_arrive(dq_empty);
       }
       if (want_table) {
-        float* other = xch + parity * 256;  // error of D per half row, its share of the last bucket
-        other[half * 128 + r] = ds_all;
-        if (!together()) break;
-        const float off = other[r] + other[128 + r];
+        const float off = row_sum(ds_all);  // the error of D
+        // what belongs to the last bucket in tiles that were summed by diagonals is in the bins already, and so is its error
         const float last = warp_sum(ds_far - off * p_far);
-        // the far part of tiles that were summed by diagonals is in the bins already, with its error: p_far covers it
         if (lane == 0) my_bins[a.buckets - 1] += last;
-        if (!together()) break;
-        parity ^= 1;
-        for (int b = threadIdx.x; b < a.buckets; b += 256) {
+        together();
+        for (int b = threadIdx.x; b < a.buckets; b += kComputeWarps * 32) {
           float sum = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < kComputeWarps; ++k) {
             sum += bins[k * kMaxBuckets + b];
             bins[k * kMaxBuckets + b] = 0.f;
           }
           p.dtable_part[((static_cast<long long>(w.b) * a.Hq + w.h) * p.n_qt + w.q0 / 128) * a.buckets + b] = sum;
         }
-        if (!together()) break;
+        together();
       }
     }
   }
@@ -1125,7 +1394,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dq_kernel(const _
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1145,8 +1414,9 @@ struct BandDkvSmem {
   static constexpr int kRing = 2 * kTile;
   static constexpr int kStat = kRing + 2 * kStages * kTile;
   static constexpr int kBar = kStat + kStages * kStatBlock * 4;
-  static constexpr int kNumBars = 2 * kStages + 11;
+  static constexpr int kNumBars = 2 * kStages + 9;
   static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;
+  static constexpr int kCols = D == 96 ? 32 : D / 4;  // as in the dQ kernel
 };
 
 struct DkvItem {
@@ -1211,27 +1481,25 @@ struct DkvWalk {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const __grid_constant__ BandBwdParams p) {
+__global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __grid_constant__ BandBwdParams p) {
   using L = BandDkvSmem<D>;
   constexpr int NS = L::kSlabs, ST = L::kStages;
   constexpr bool kOwn = D == 64;  // P^T and dS^T have their own columns
   constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D, kP = kOwn ? 384 : 0, kDs = kOwn ? 448 : 128;
-  constexpr uint32_t kHalf = kOwn ? 32 : 64;  // a warp that is ahead must not write over the half that another still reads
+  constexpr int kQuarter = kOwn ? 16 : 32;  // a warp that is ahead must not write over what another still reads
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* q_full = bars;             // [ST]
-  uint64_t* q_empty = bars + ST;       // [ST] dK of the step issued and done + 8 warps that read the statistics
+  uint64_t* q_empty = bars + ST;       // [ST] both issuers + the warps that read the statistics
   uint64_t* kv_full = bars + 2 * ST;
-  uint64_t* kv_empty = kv_full + 1;
+  uint64_t* kv_empty = kv_full + 1;    // both issuers, as for acc_full
   uint64_t* s_full = kv_full + 2;
   uint64_t* s_read = kv_full + 3;
   uint64_t* dp_full = kv_full + 4;
-  uint64_t* dp_read = kv_full + 5;
-  uint64_t* p_full = kv_full + 6;
-  uint64_t* ds_full = kv_full + 7;
-  uint64_t* acc_full = kv_full + 8;
-  uint64_t* acc_empty = kv_full + 9;
-  uint64_t* sync_bar = kv_full + 10;
+  uint64_t* p_full = kv_full + 5;
+  uint64_t* ds_full = kv_full + 6;
+  uint64_t* acc_full = kv_full + 7;
+  uint64_t* acc_empty = kv_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const BandArgs& a = p.a;
@@ -1247,37 +1515,40 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 9);
+      mbar_init(&q_empty[s], 2 + kComputeWarps);
     }
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 1);
+    mbar_init(kv_empty, 2);
     mbar_init(s_full, 1);
-    mbar_init(s_read, 8);
+    mbar_init(s_read, kComputeWarps);
     mbar_init(dp_full, 1);
-    mbar_init(dp_read, 8);
-    mbar_init(p_full, 8);
-    mbar_init(ds_full, 8);
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 8);
-    mbar_init(sync_bar, 8);
+    mbar_init(p_full, kComputeWarps);
+    mbar_init(ds_full, kComputeWarps);
+    mbar_init(acc_full, kOwn ? 1 : 2);
+    mbar_init(acc_empty, kComputeWarps);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (a.table != nullptr) build_bucket_map(a, p.t_last, map, threadIdx.x, kBwdBandThreads);
+  if (a.table != nullptr) build_bucket_map(a, p.t_last, map, threadIdx.x, kBandThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // All 512 columns were allocated, so they begin at 0; said as a constant the addresses need no moves to uniform registers.
+  constexpr uint32_t tmem = 0;
+  if (threadIdx.x == 0 && *tmem_slot != 0) {
+    report_status(a.status, kBadArgument, 75);
+    *abort_flag = 1;
+  }
   pdl_enter();
   const int group = a.Hq / a.Hkv;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8 && lane == 0) {
+  if (warp >= kComputeWarps) {
+    NMB_BAND_FEW_REGISTERS;
+    if (warp == kLoadWarp && lane == 0) {
       // ---------------------------------------------------------- producer --
       tma_prefetch_desc(&p.q_map);
       tma_prefetch_desc(&p.do_map);
@@ -1288,7 +1559,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
       int n = 0, n_item = 0;
       for (bool more = x.open(p, 0); more; more = x.next(p), ++n) {
         if (x.first()) {
-          if (n_item > 0 && !mbar_wait(kv_empty, (n_item - 1) & 1, abort_flag, a.status, 101)) break;
+          if (n_item > 0 && !band_wait(kv_empty, (n_item - 1) & 1, abort_flag, a.status, 101)) break;
           ++n_item;
           mbar_expect_tx(kv_full, 2 * L::kTile);
 #pragma unroll
@@ -1298,7 +1569,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
           }
         }
         const int st = n % ST, use = n / ST;
-        if (use > 0 && !mbar_wait(&q_empty[st], (use - 1) & 1, abort_flag, a.status, 102)) break;
+        if (use > 0 && !band_wait(&q_empty[st], (use - 1) & 1, abort_flag, a.status, 102)) break;
         const int h = x.w.hk * group + x.step / x.w.per_head, qt = x.w.first_qt + x.step % x.w.per_head;
         mbar_expect_tx(&q_full[st], 2 * L::kTile + stat_bytes);
 #pragma unroll
@@ -1310,73 +1581,68 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
         bulk_load(smem + L::kStat + st * kStatBlock * 4,
                   p.stat + ((static_cast<long long>(x.w.b) * a.Hq + h) * p.n_qt + qt) * kStatBlock, stat_bytes, &q_full[st]);
       }
-    } else if (warp == 9) {
-      // -------------------------------------------------------- MMA issuer --
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+      // ------------------------------------------------------- MMA issuers --
+      // Columns that are written by one product and read by another as operand stay with one issuer, whose products run in
+      // order: S^T and, where P^T overwrites it, dV with the first; dP^T and dK (and else dV) with the second.  So dP^T of a
+      // step is complete after dK (and dV) of the step before, and S^T after dV of the step before where that matters.
       constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t idesc_d = make_idesc_bf16(128, D, false, true);
       const uint32_t sk = smem_u32(smem + L::kK), ring = smem_u32(smem + L::kRing);
-      const uint32_t k_low = desc_k(sk), v_low = desc_k(sk + L::kTile);
       const bool one = elect_one();
+      const bool is_s = warp == kMmaWarp;
+      const uint32_t a_low = desc_k(is_s ? sk : sk + L::kTile), d = is_s ? tmem : tmem + kDp, b_off = is_s ? 0 : L::kTile;
       DkvWalk x;
       uint32_t n = 0, n_item = 0;  // step, item of `x`
       bool more = x.open(p, 0);
-      bool ok = more && warp_wait(kv_full, 0, abort_flag, a.status, 103) && warp_wait(&q_full[0], 0, abort_flag, a.status, 104);
-      if (ok) {
+      // S^T or dP^T of a step
+      auto scores = [&](uint32_t n, bool last) {
         tc_fence_after();
-        const bool last = x.last();
         if (one) {
-          mma_scores<D>(tmem, k_low, desc_k(ring), idesc_s);
-          tc_commit(s_full);
-          mma_scores<D>(tmem + kDp, v_low, desc_k(ring + L::kTile), idesc_s);
-          tc_commit(dp_full);
+          mma_scores<D>(d, a_low, desc_k(ring + 2 * (n % ST) * L::kTile + b_off), idesc_s);
+          tc_commit(is_s ? s_full : dp_full);
           if (last) tc_commit(kv_empty);
         }
-      }
+      };
+      bool ok = more && band_wait(kv_full, 0, abort_flag, a.status, 103) && band_wait(&q_full[0], 0, abort_flag, a.status, 104);
+      if (ok) scores(0, x.last());
       while (ok && more) {
         DkvWalk y = x;
         const bool ahead = y.next(p), fresh = ahead && y.first(), y_last = ahead && y.last();
         const bool x_first = x.first(), x_last = x.last();
-        const uint32_t n_item2 = n_item + fresh;
-        const uint32_t sq = ring + 2 * (n % ST) * L::kTile, sq2 = ring + 2 * ((n + 1) % ST) * L::kTile;
-        // S^T and dP^T of the next step
-        auto next_s = [&]() {
-          if (!ahead) return true;
-          if (fresh && !warp_wait(kv_full, n_item2 & 1, abort_flag, a.status, 105)) return false;
-          if (!warp_wait(&q_full[(n + 1) % ST], ((n + 1) / ST) & 1, abort_flag, a.status, 106)) return false;
-          if (kOwn && !warp_wait(s_read, n & 1, abort_flag, a.status, 107)) return false;
-          tc_fence_after();
-          if (one) {
-            mma_scores<D>(tmem, k_low, desc_k(sq2), idesc_s);
-            tc_commit(s_full);
-          }
-          return true;
+        const uint32_t n_item2 = n_item + fresh, sq = ring + 2 * (n % ST) * L::kTile;
+        // what the next step's scores need; looked for while the products of this step run
+        auto next_there = [&]() {
+          return (!fresh || band_wait(kv_full, n_item2 & 1, abort_flag, a.status, 105)) &&
+                 band_wait(&q_full[(n + 1) % ST], ((n + 1) / ST) & 1, abort_flag, a.status, 106);
         };
-        auto next_dp = [&]() {
-          if (one) {
-            mma_scores<D>(tmem + kDp, v_low, desc_k(sq2 + L::kTile), idesc_s);
-            tc_commit(dp_full);
-            if (y_last) tc_commit(kv_empty);
+        if (kOwn && is_s) {
+          if (ahead) {
+            if (!next_there() || !band_wait(s_read, n & 1, abort_flag, a.status, 107)) break;
+            scores(n + 1, y_last);
           }
-        };
-        if (kOwn && !next_s()) break;
-        if (x_first && n_item > 0 && !warp_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
-        if (!warp_wait(p_full, n & 1, abort_flag, a.status, 109)) break;
-        tc_fence_after();
-        if (one) mma_apply<kHalf>(tmem + kDv, tmem + kP, desc_mn(sq + L::kTile), idesc_d, x_first);
-        if (!kOwn && !next_s()) break;
-        if (kOwn && ahead) {
-          if (!warp_wait(dp_read, n & 1, abort_flag, a.status, 110)) break;
-          tc_fence_after();
-          next_dp();
+          if (one) tc_commit(&q_empty[n % ST]);
+        } else {
+          if (x_first && n_item > 0 && !band_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
+          if (kOwn || is_s) {
+            if (!band_wait(p_full, n & 1, abort_flag, a.status, 109)) break;
+            tc_fence_after();
+            if (one) mma_apply<8, 2, kQuarter>(tmem + kDv, tmem + kP, desc_mn(sq + L::kTile), idesc_d, x_first);
+          }
+          if (!is_s) {
+            if (!band_wait(ds_full, n & 1, abort_flag, a.status, 111)) break;
+            tc_fence_after();
+            if (one) mma_apply<8, 2, kQuarter>(tmem + kDk, tmem + kDs, desc_mn(sq), idesc_d, x_first);
+          }
+          if (one) {
+            tc_commit(&q_empty[n % ST]);
+            if (x_last) tc_commit(acc_full);
+          }
+          if (ahead) {
+            if (!next_there()) break;
+            scores(n + 1, y_last);
+          }
         }
-        if (!warp_wait(ds_full, n & 1, abort_flag, a.status, 111)) break;
-        tc_fence_after();
-        if (one) {
-          mma_apply<kHalf>(tmem + kDk, tmem + kDs, desc_mn(sq), idesc_d, x_first);
-          tc_commit(&q_empty[n % ST]);
-          if (x_last) tc_commit(acc_full);
-        }
-        if (!kOwn && ahead) next_dp();
         x = y;
         more = ahead;
         n_item = n_item2;
@@ -1384,18 +1650,18 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    NMB_BAND_MORE_REGISTERS;
     // ------------------------------------------------------------ compute --
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, quarter = warp >> 2;
     const int r = quad * 32 + lane;  // key of the tile == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const bool has_cols = quarter * L::kCols < D;
     const float sl2 = a.scale * kBandLog2e;
     const int rounds = (p.n_items + gridDim.x - 1) / gridDim.x;
     int n = 0, n_item = 0;
-    uint32_t sync_phase = 0;
-    auto together = [&]() { return group_sync(sync_bar, sync_phase, abort_flag, a.status, 118); };
+    auto together = [&]() { named_sync(1, kComputeWarps * 32); };
     bool ok = true;
-    for (int round = 0; round < rounds && ok; ++round) {
+    for (int round = 0; round < rounds; ++round) {
       const int item = item_of_round(round);
       if (item >= p.n_items) continue;
       const DkvItem w = dkv_item(p, item);
@@ -1407,113 +1673,72 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
         const int pmin = a.q_pos0 + qt * 128;
         const int st = n % ST;
         if (a.table != nullptr && h != lut_h) {
-          ok = together();  // everyone is done with the table of the head before
-          build_lut(a, h, p.t_last, map, lut, threadIdx.x, 256);
-          ok = ok && together();
-          if (!ok) break;
+          together();  // everyone is done with the table of the head before
+          build_lut(a, h, p.t_last, map, lut, threadIdx.x, kComputeWarps * 32);
+          together();
           far_bias = lut[entries - 1];
           lut_h = h;
         }
         // the statistics come with Q and dO; the scores do after them
-        if (!warp_wait(&q_full[st], (n / ST) & 1, abort_flag, a.status, 112) ||
-            !warp_wait(s_full, n & 1, abort_flag, a.status, 113)) {
-          ok = false;
-          break;
-        }
+        NMB_BAND_WAIT(&q_full[st], (n / ST) & 1, 112);
+        NMB_BAND_WAIT(s_full, n & 1, 113);
         tc_fence_after();
-        uint32_t s[2][32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld_32x32(t_row + half * 64 + c * 32, s[c]);
+        uint32_t s[32];
+        tmem_ld_32x32(t_row + quarter * 32, s);
         tmem_ld_wait();
         if (kOwn) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(s_read);
         }
-        const float* stat = reinterpret_cast<const float*>(smem + L::kStat) + st * kStatBlock + half * 64;
+        const float* stat = reinterpret_cast<const float*>(smem + L::kStat) + st * kStatBlock + quarter * 32;
         const bool added = a.table != nullptr && (pmin - (w.kv0 + 127) < p.t_last || fabsf(far_bias) > 1e30f);
         const bool whole = w.kv0 + 127 <= pmin && w.kv0 + 127 < a.Skv && (pmin + 127 - w.kv0 < a.window || w.kv0 + 127 < a.sinks);
-        if (!added) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 cc = *reinterpret_cast<const float4*>(stat + c * 32 + k);
-              s[c][k] = __float_as_uint(ex2(fmaf(__uint_as_float(s[c][k]), sl2, cc.x)));
-              s[c][k + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(s[c][k + 1]), sl2, cc.y)));
-              s[c][k + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(s[c][k + 2]), sl2, cc.z)));
-              s[c][k + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(s[c][k + 3]), sl2, cc.w)));
-            }
+        if (whole && !added && qt * 128 + 128 <= a.Sq) {  // as in the dQ kernel
+          exps32<true>(s, pack2(sl2, sl2), stat);
+        } else if (!added) {
+          exps32<false>(s, pack2(sl2, sl2), stat);
         } else {
-          const float* at = lut + kLutFront + min(pmin - j, p.t_last + 128) + half * 64;
+          const float* at = lut + kLutFront + min(pmin - j, p.t_last + 128) + quarter * 32;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              s[c][k] = __float_as_uint(
-                  ex2((fmaf(__uint_as_float(s[c][k]), sl2, at[c * 32 + k]) - stat[256 + c * 32 + k]) - stat[384 + c * 32 + k]));
+          for (int k = 0; k < 32; ++k)
+            s[k] = __float_as_uint(ex2((fmaf(__uint_as_float(s[k]), sl2, at[k]) - stat[256 + k]) - stat[384 + k]));
         }
         if (!whole) {
-          const int lo = j < a.Skv ? j - pmin : 128, hi = j < a.sinks ? 128 : j - pmin + a.window;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int c0 = half * 64 + c * 32;
-            const uint32_t see = low_bits(hi - c0) & ~low_bits(lo - c0);
+          const int c0 = quarter * 32, lo = j < a.Skv ? j - pmin : 128, hi = j < a.sinks ? 128 : j - pmin + a.window;
+          const uint32_t see = low_bits(hi - c0) & ~low_bits(lo - c0);
+          if (!__all_sync(0xffffffffu, see == ~0u)) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (!((see >> k) & 1u)) s[c][k] = 0;
+              if (!((see >> k) & 1u)) s[k] = 0;
           }
         }
-        if (kOwn && !warp_wait(dp_full, n & 1, abort_flag, a.status, 114)) {  // P^T of the step before has been read
-          ok = false;
-          break;
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        if (kOwn) NMB_BAND_WAIT(dp_full, n & 1, 114);  // P^T and dS^T of the step before have been read
+        {
           uint32_t pk[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) pk[k] = pack_bf16x2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
-          tmem_st_32x16(t_row + kP + half * kHalf + c * 16, pk);
+          for (int k = 0; k < 16; ++k) pk[k] = pack_bf16x2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+          tmem_st_32x16(t_row + kP + quarter * kQuarter, pk);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
-        if (!kOwn && !warp_wait(dp_full, n & 1, abort_flag, a.status, 115)) {
-          ok = false;
-          break;
-        }
+        if (!kOwn) NMB_BAND_WAIT(dp_full, n & 1, 115);
         tc_fence_after();
-        uint32_t dp[2][32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld_32x32(t_row + kDp + half * 64 + c * 32, dp[c]);
+        uint32_t dp[32];
+        tmem_ld_32x32(t_row + kDp + quarter * 32, dp);
         tmem_ld_wait();
-        if (kOwn) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(dp_read);
+        uint32_t pk[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 dd = *reinterpret_cast<const float4*>(stat + 128 + k);
+          pk[k / 2] = pack_bf16x2(__uint_as_float(s[k]) * (__uint_as_float(dp[k]) - dd.x),
+                                  __uint_as_float(s[k + 1]) * (__uint_as_float(dp[k + 1]) - dd.y));
+          pk[k / 2 + 1] = pack_bf16x2(__uint_as_float(s[k + 2]) * (__uint_as_float(dp[k + 2]) - dd.z),
+                                      __uint_as_float(s[k + 3]) * (__uint_as_float(dp[k + 3]) - dd.w));
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 dd = *reinterpret_cast<const float4*>(stat + 128 + c * 32 + k);
-            s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * (__uint_as_float(dp[c][k]) - dd.x));
-            s[c][k + 1] = __float_as_uint(__uint_as_float(s[c][k + 1]) * (__uint_as_float(dp[c][k + 1]) - dd.y));
-            s[c][k + 2] = __float_as_uint(__uint_as_float(s[c][k + 2]) * (__uint_as_float(dp[c][k + 2]) - dd.z));
-            s[c][k + 3] = __float_as_uint(__uint_as_float(s[c][k + 3]) * (__uint_as_float(dp[c][k + 3]) - dd.w));
-          }
-        if (kOwn && n > 0 && !warp_wait(&q_empty[(n - 1) % ST], ((n - 1) / ST) & 1, abort_flag, a.status, 116)) {
-          ok = false;  // dS^T of the step before has been read
-          break;
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) pk[k] = pack_bf16x2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
-          tmem_st_32x16(t_row + kDs + half * kHalf + c * 16, pk);
-        }
+        tmem_st_32x16(t_row + kDs + quarter * kQuarter, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -1522,33 +1747,34 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
           mbar_arrive(&q_empty[st]);
         }
       }
-      if (!ok) break;
       const bool any = w.from < w.to;
       if (any) {
-        if (!warp_wait(acc_full, n_item & 1, abort_flag, a.status, 117)) break;
+        NMB_BAND_WAIT(acc_full, n_item & 1, 117);
         ++n_item;
         tc_fence_after();
       }
+      if (has_cols) {
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const float mul = which == 0 ? 1.f : a.scale;
-        __nv_bfloat16* out = band_row(which == 0 ? a.dv : a.dk, which == 0 ? a.dv_st : a.dk_st, w.b, j, w.hk) + half * (D / 2);
-        float* part = p.part + ((static_cast<long long>(w.slot) * 2 + which) * 128 + r) * D + half * (D / 2);
+        for (int which = 0; which < 2; ++which) {
+          const float mul = which == 0 ? 1.f : a.scale;
+          __nv_bfloat16* out = band_row(which == 0 ? a.dv : a.dk, which == 0 ? a.dv_st : a.dk_st, w.b, j, w.hk) + quarter * L::kCols;
+          float* part = p.part + ((static_cast<long long>(w.slot) * 2 + which) * 128 + r) * D + quarter * L::kCols;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[16];
-          if (any) {
-            tmem_ld_32x16(t_row + (which == 0 ? kDv : kDk) + half * (D / 2) + c * 16, v);
-            tmem_ld_wait();
-          } else {
+          for (int c = 0; c < L::kCols / 16; ++c) {
+            uint32_t v[16];
+            if (any) {
+              tmem_ld_32x16(t_row + (which == 0 ? kDv : kDk) + quarter * L::kCols + c * 16, v);
+              tmem_ld_wait();
+            } else {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = 0;
-          }
-          if (w.slot >= 0) {
-            st_global_32(part + c * 16, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
-            st_global_32(part + c * 16 + 8, v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]);
-          } else if (j < a.Skv) {
-            store_bf16_16(out + c * 16, v, mul);
+              for (int k = 0; k < 16; ++k) v[k] = 0;
+            }
+            if (w.slot >= 0) {
+              st_global_32(part + c * 16, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+              st_global_32(part + c * 16 + 8, v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]);
+            } else if (j < a.Skv) {
+              store_bf16_16(out + c * 16, v, mul);
+            }
           }
         }
       }
@@ -1565,7 +1791,7 @@ __global__ void __launch_bounds__(kBwdBandThreads, 1) band_bwd_dkv_kernel(const 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1694,11 +1920,11 @@ template <int D>
 static cudaError_t launch_band_bwd(BandBwdParams& p, long long dq_items, long long dkv_items, bool split, cudaStream_t s) {
   const int lut = p.a.table == nullptr ? 0 : lut_bytes(p.t_last, 1);
   p.n_items = static_cast<int>(dq_items);
-  cudaError_t e = launch_pdl(band_bwd_dq_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBwdBandThreads),
+  cudaError_t e = launch_pdl(band_bwd_dq_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads),
                              BandDqSmem<D>::kLut + lut + (p.a.dtable == nullptr ? 0 : BandDqSmem<D>::kBins), s, p);
   if (e != cudaSuccess) return e;
   p.n_items = static_cast<int>(dkv_items);
-  e = launch_pdl(band_bwd_dkv_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBwdBandThreads),
+  e = launch_pdl(band_bwd_dkv_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads),
                  BandDkvSmem<D>::kLut + lut, s, p);
   const int tiles = !split ? 0 : (p.pieces > 1 ? p.n_kt : p.sink_tiles) - (p.sink_pieces > 1 ? 0 : p.sink_tiles);
   const long long sum_blocks = static_cast<long long>(tiles) * p.a.Hkv * p.a.B * (D / 8);  // 2 * 128 rows of D / 8 octets, 256 a block
