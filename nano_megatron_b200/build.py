@@ -1,4 +1,4 @@
-"""Ahead-of-time build of the sm_100a kernel library.
+"""Ahead-of-time build of the sm_100a kernel library and of the C++ autograd operators on top of it.
 
 Every ``csrc/*.cu`` file is compiled with ``nvcc -gencode
 arch=compute_100a,code=sm_100a`` into an object file and the objects are linked
@@ -25,6 +25,7 @@ PKG_DIR = Path(__file__).resolve().parent
 SRC_DIR = PKG_DIR / "csrc"
 OBJ_DIR = PKG_DIR / "csrc" / "build"
 LIB_PATH = PKG_DIR / "libnmb_kernels.so"
+TORCH_LIB_PATH = PKG_DIR / "libnmb_torch.so"   # autograd operators in C++, on top of the kernel library
 
 NVCC_FLAGS = [
     "-gencode",
@@ -69,6 +70,27 @@ def _compile_one(src: Path, force: bool) -> tuple[Path, str]:
     return obj, proc.stderr
 
 
+def _build_torch_binding(force: bool) -> None:
+    """``csrc/torch_binding.cpp`` -> ``libnmb_torch.so``, with the host compiler and PyTorch's own headers."""
+    import torch
+    from torch.utils import cpp_extension
+
+    src, stamp = SRC_DIR / "torch_binding.cpp", OBJ_DIR / "torch_binding.sha"
+    digest = hashlib.sha256((_digest(src) + torch.__version__).encode()).hexdigest()
+    if not force and TORCH_LIB_PATH.exists() and stamp.exists() and stamp.read_text() == digest:
+        return
+    cuda = Path(_nvcc()).resolve().parent.parent
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-isystem{p}" for p in (*cpp_extension.include_paths(), cuda / "include")], str(src), "-o", str(TORCH_LIB_PATH),
+           str(LIB_PATH), f"-L{lib}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{src.name} failed:\n{proc.stdout}\n{proc.stderr}")
+    stamp.write_text(digest)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile and link the kernel library; returns its path."""
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
@@ -84,10 +106,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if log:
             logs.append(f"==== {src.name}\n{log}")
     if rebuilt or force or not LIB_PATH.exists():
-        cmd = [_nvcc(), "-shared", "-o", str(LIB_PATH), *objs, "-lcudart"]
+        cmd = [_nvcc(), "-shared", "-o", str(LIB_PATH), *objs, "-lcudart", "-Xlinker", "-soname=libnmb_kernels.so"]
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
+    _build_torch_binding(force)
     if logs:
         (OBJ_DIR / "ptxas.log").write_text("\n".join(logs))
         if verbose:

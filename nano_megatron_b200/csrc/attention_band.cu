@@ -9,42 +9,16 @@
 //   dQ = scale dS K,  dK = scale dS^T Q,  dtable[h, b] = sum of dS_ij with bucket(p_i - j) = b
 // Rows are kept by their maximum m and l = log2(sum 2^(x - m)), both in the base-2 exponent domain and apart
 // from one another: with a bias of the type's lowest value in every place m + l would round l away.
+#include "band_args.h"
 #include "common.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace nmb {
 
 constexpr float kBandLog2e = 1.4426950408889634f;
-constexpr int kMaxBuckets = 128;
-constexpr int kMaxDistance = 2048;
 constexpr float kBiasLimit = 3.0e38f;  // finite biases stay finite after the change to base 2
-
-struct BandStride {
-  long long b, s, h;  // elements; head_dim is contiguous
-};
-
-// Arguments of both passes, laid out as in ops/band_attention.py: the pointers of a call, then what its shapes fix.
-struct BandArgs {
-  const __nv_bfloat16 *q, *k, *v;
-  __nv_bfloat16* o;
-  const __nv_bfloat16* dout;
-  __nv_bfloat16 *dq, *dk, *dv;
-  float* m;              // [B, Hq, Sq]
-  float* l;              // [B, Hq, Sq]
-  float* scratch;        // nmb_band_bwd_scratch() floats, backward only
-  const void* table;     // [Hq, buckets] bf16 or fp32; null without a bias
-  void* dtable;          // [Hq, buckets]; null when it is not wanted
-  int* status;
-  int table_fp32, dtable_fp32, accumulate;  // accumulate: dtable is added to
-  int pad;
-  BandStride q_st, k_st, v_st, o_st, dout_st, dq_st, dk_st, dv_st;
-  int B, Hq, Hkv, Sq, Skv, d;
-  int q_pos0, window, sinks, buckets;
-  float scale;
-  int pad2;
-  unsigned short limit[kMaxBuckets];  // first distance of bucket b + 1
-};
 
 __device__ __forceinline__ float table_at(const BandArgs& p, int h, int b) {
   const long long at = static_cast<long long>(h) * p.buckets + b;
@@ -1815,10 +1789,10 @@ __global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant_
     if (lane == 0) {
       if (a.dtable_fp32) {
         float* out = static_cast<float*>(a.dtable) + at;
-        *out = a.accumulate ? *out + acc : acc;
+        *out = acc;
       } else {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.dtable) + at;
-        *out = __float2bfloat16(a.accumulate ? __bfloat162float(*out) + acc : acc);
+        *out = __float2bfloat16(acc);
       }
     }
     return;
@@ -1939,6 +1913,10 @@ static cudaError_t launch_band_bwd(BandBwdParams& p, long long dq_items, long lo
 
 using namespace nmb;
 
+static std::atomic<long long> g_band_launches{0};
+
+extern "C" long long nmb_band_launches() { return g_band_launches.load(); }
+
 static int band_check(const BandArgs* a) {
   if (a->d != 64 && a->d != 96 && a->d != 128) return kBadArgument;
   if (a->B < 1 || a->Hkv < 1 || a->Hq % a->Hkv != 0 || a->Sq < 1 || a->Skv < 1) return kBadArgument;
@@ -1957,7 +1935,6 @@ static int band_check(const BandArgs* a) {
 
 extern "C" int nmb_band_args_size() { return static_cast<int>(sizeof(BandArgs)); }
 
-// Floats of `scratch` that the backward pass of these arguments needs.
 extern "C" long long nmb_band_bwd_scratch(const BandArgs* a) {
   if (band_check(a)) return 0;
   BandBwdParams p;
@@ -2004,6 +1981,7 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   p.n_items = static_cast<int>(items);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = a->d == 64 ? launch_band_fwd<64>(p, s) : a->d == 96 ? launch_band_fwd<96>(p, s) : launch_band_fwd<128>(p, s);
+  if (e == cudaSuccess) ++g_band_launches;
   return e == cudaSuccess ? 0 : 400 + e;
 }
 
@@ -2029,5 +2007,6 @@ extern "C" int nmb_band_bwd(const BandArgs* a, void* stream) {
   const cudaError_t e = a->d == 64 ? launch_band_bwd<64>(p, dq_items, dkv_items, split, s)
                       : a->d == 96 ? launch_band_bwd<96>(p, dq_items, dkv_items, split, s)
                                    : launch_band_bwd<128>(p, dq_items, dkv_items, split, s);
+  if (e == cudaSuccess) g_band_launches += 2 + (split || a->dtable != nullptr);
   return e == cudaSuccess ? 0 : 500 + e;
 }

@@ -98,10 +98,8 @@ def lib() -> ctypes.CDLL:
                         "(the CUDA ops do not fall back to PyTorch on a GPU)"
                     )
                 _lib = ctypes.CDLL(str(_LIB_PATH))
-                for fn in (_lib.nmb_band_fwd, _lib.nmb_band_bwd):
-                    fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]   # packed arguments, stream
-                _lib.nmb_band_bwd_scratch.argtypes = [ctypes.c_char_p]
                 _lib.nmb_band_bwd_scratch.restype = ctypes.c_longlong
+                _lib.nmb_band_launches.restype = ctypes.c_longlong
                 pair = os.environ.get("NMB_GEMM_PAIR")
                 if pair is not None:
                     _lib.nmb_gemm_set_pair(int(pair != "0"))
@@ -110,6 +108,24 @@ def lib() -> ctypes.CDLL:
                     _lib.nmb_set_pdl(int(pdl != "0"))
     _configure_current_device(_lib)
     return _lib
+
+
+_torch_lib_loaded = False
+
+
+def torch_lib():
+    """The operators of ``libnmb_torch.so`` (autograd functions in C++), as ``torch.ops.nmb``."""
+    global _torch_lib_loaded
+    if not _torch_lib_loaded:
+        lib()
+        with _lock:
+            if not _torch_lib_loaded:
+                path = _LIB_PATH.with_name("libnmb_torch.so")
+                if not path.exists():
+                    raise NativeKernelError(f"{path} is missing: run `python -m nano_megatron_b200.build`")
+                torch.ops.load_library(str(path))
+                _torch_lib_loaded = True
+    return torch.ops.nmb
 
 
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -149,8 +165,9 @@ def check_status(device: torch.device | None = None, *, reset: bool = True) -> N
 
 
 #: kernels launched by each C entry point (for launch accounting)
-_KERNELS_PER_CALL = {"nmb_attn_bwd": 3, "nmb_band_bwd": 2, "nmb_col_reduce": 2, "nmb_adamw_step": 2}
-#: running count of kernels of this library launched (or captured) by this process
+_KERNELS_PER_CALL = {"nmb_attn_bwd": 3, "nmb_col_reduce": 2, "nmb_adamw_step": 2}
+#: running count of kernels of this library launched (or captured) by this process through the wrappers of this package; the
+#: banded attention is launched from C++ and counts its own (``nmb_band_launches``)
 launches = 0
 #: the same per C entry point (tests use it to show that a fused path left no stand-alone kernel behind)
 launch_counts: dict[str, int] = {}

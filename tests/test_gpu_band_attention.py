@@ -1,6 +1,7 @@
 """The banded attention kernels against the definition in 64 bits."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -9,6 +10,28 @@ import torch
 from tests._band_oracle import check, oracle
 
 pytestmark = pytest.mark.gpu
+
+
+class _Stride(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_longlong) for n in "bsh"]
+
+
+_TENSORS = ("q", "k", "v", "o", "dout", "dq", "dk", "dv")
+
+
+class _Args(ctypes.Structure):
+    """BandArgs of csrc/band_args.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in (*_TENSORS, "m", "l", "scratch", "table", "dtable", "status")]
+                + [(n + "_st", _Stride) for n in _TENSORS]
+                + [(n, ctypes.c_int) for n in ("table_fp32", "dtable_fp32", "B", "Hq", "Hkv", "Sq", "Skv", "d", "q_pos0", "window",
+                                               "sinks", "buckets")]
+                + [("scale", ctypes.c_float), ("pad", ctypes.c_int), ("limit", ctypes.c_ushort * 128)])
+
+
+def _launches():
+    from nano_megatron_b200.ops import native
+
+    return native.lib().nmb_band_launches()
 
 
 def _tensors(b, sq, skv, hq, hkv, d, buckets=0, layout="bshd", seed=0, table_dtype=torch.bfloat16, gain=1.0):
@@ -49,13 +72,13 @@ def _compare(q, k, v, table, dout, *, window=None, sinks=0, start=0, max_distanc
     from nano_megatron_b200.ops import native
 
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-    before = native.launch_counts.get("nmb_band_bwd", 0)
+    before = _launches()
     out = _call(q, k, v, table, scale, max_distance, window=window, sinks=sinks, query_start=start)
     leaves = [q, k, v] + ([] if table is None else [table])
     grads = torch.autograd.grad(out, leaves, dout)
     torch.cuda.synchronize()
     native.check_status()
-    assert native.launch_counts["nmb_band_bwd"] == before + 1  # the kernels ran
+    assert _launches() >= before + 3  # the kernels ran: forward, dQ, dK and dV
     values, bounds, rms = oracle(q, k, v, dout, scale, window=window, sinks=sinks, start=start, table=table, max_distance=max_distance)
     check(dict(zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads))), values, bounds, rms, what)
 
@@ -177,6 +200,7 @@ def test_main_grad_of_the_table():
         param._nmb_grad_ready = lambda: ready.append(1)
         relative_bias_attention(q, k, v, param, 0.125, max_distance=60).backward(dout)
         torch.testing.assert_close(buffer, want + 1, rtol=1e-6, atol=1e-6)
+        assert param.grad is None
         param._nmb_overwrite_next = True
         relative_bias_attention(q, k, v, param, 0.125, max_distance=60).backward(dout)
         torch.testing.assert_close(buffer, want, rtol=0, atol=0)
@@ -244,6 +268,8 @@ def test_nothing_is_written_outside(sq, skv, d, start, buckets):
     b, hq, hkv, pad = 2, 4, 2, 9
     q, k, v, table, dout = (None if t is None else t.detach() for t in _tensors(b, sq, skv, hq, hkv, d, buckets))
     mark = 7.0
+    lib = native.lib()
+    assert lib.nmb_band_args_size() == ctypes.sizeof(_Args)
 
     def inside(s, h):
         big = torch.full((b, s + 2 * pad, h, d), mark, device="cuda", dtype=torch.bfloat16)
@@ -255,26 +281,22 @@ def test_nothing_is_written_outside(sq, skv, d, start, buckets):
 
     bufs = {n: inside(s, h) for n, s, h in (("o", sq, hq), ("dq", sq, hq), ("dk", skv, hkv), ("dv", skv, hkv))}
     stats = {n: flat(b * hq * sq) for n in ("m", "l")}
-    lib = native.lib()
-    p = ba._plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), True, buckets or None, 128, 0.125, 50, 3, start)
     if buckets:
         stats["dtable"] = flat(hq * buckets)
-    stats["scratch"] = flat(ba._scratch(p, lib))
-    views = {n: t[1] for n, t in {**bufs, **stats}.items()}
-
-    def at(n):
-        return views[n].data_ptr() if n in views else 0
-
-    # the same strides but for the batch: rows of larger buffers
-    fixed = list(ba._FIXED.unpack(p.bwd))
-    for n, i in (("o", 3), ("dq", 5), ("dk", 6), ("dv", 7)):
-        fixed[3 * i] = views[n].stride(0)
-    args = ba._POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), at("o"), dout.data_ptr(), at("dq"), at("dk"), at("dv"), at("m"),
-                             at("l"), at("scratch"), 0 if table is None else table.data_ptr(), at("dtable"),
-                             native.status_word(q.device).data_ptr(), 0, 1, 0, 0) + ba._FIXED.pack(*fixed)
-    stream = torch.cuda.current_stream().cuda_stream
-    native.check_rc(lib.nmb_band_fwd(args, stream), "nmb_band_fwd")
-    native.check_rc(lib.nmb_band_bwd(args, stream), "nmb_band_bwd")
+    args = _Args(B=b, Hq=hq, Hkv=hkv, Sq=sq, Skv=skv, d=d, q_pos0=start, window=50, sinks=3, buckets=buckets, scale=0.125, dtable_fp32=1,
+                 status=native.status_word(q.device).data_ptr(), table=None if table is None else table.data_ptr())
+    if buckets:
+        args.limit[:buckets - 1] = ba.relative_bucket_limits(buckets, 128)
+    views = {n: t[1] for n, t in {**bufs, **stats}.items()} | {"q": q, "k": k, "v": v, "dout": dout}
+    for n, t in views.items():
+        setattr(args, n, t.data_ptr())
+        if n in _TENSORS:
+            setattr(args, n + "_st", _Stride(*t.stride()[:3]))
+    stats["scratch"] = flat(lib.nmb_band_bwd_scratch(ctypes.byref(args)))
+    args.scratch = stats["scratch"][1].data_ptr()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    native.check_rc(lib.nmb_band_fwd(ctypes.byref(args), stream), "nmb_band_fwd")
+    native.check_rc(lib.nmb_band_bwd(ctypes.byref(args), stream), "nmb_band_bwd")
     torch.cuda.synchronize()
     native.check_status()
     for n, (big, view) in bufs.items():
@@ -298,3 +320,28 @@ def test_tensors_of_another_device():
     q, k, v, table, dout = (t.detach().to("cuda:1").requires_grad_(True) for t in _tensors(1, 200, 200, 2, 2, 64, 32))
     with torch.cuda.device(0):
         _compare(q, k, v, table, dout)
+
+
+def test_layout_of_the_gradients():
+    from nano_megatron_b200.ops.band_attention import window_attention
+
+    for layout in ("bshd", "bhsd"):  # the inputs' own layouts
+        q, k, v, _, dout = _tensors(2, 100, 100, 4, 2, 64, layout=layout)
+        for t, g in zip((q, k, v), torch.autograd.grad(window_attention(q, k, v, 0.125, window=30), (q, k, v), dout)):
+            assert g.stride() == t.stride()
+    qkv = torch.randn(2, 100, 8 * 64, device="cuda").to(torch.bfloat16)  # one buffer for the slices of a packed projection
+    q, k, v = (t.unflatten(-1, (-1, 64)).detach().requires_grad_(True) for t in qkv.split([4 * 64, 2 * 64, 2 * 64], dim=-1))
+    dq, dk, dv = torch.autograd.grad(window_attention(q, k, v, 0.125, window=30), (q, k, v), torch.ones(2, 100, 4, 64, device="cuda", dtype=torch.bfloat16))
+    assert dq.stride() == q.stride() and dk.data_ptr() == dq.data_ptr() + 2 * 4 * 64 and dv.data_ptr() == dk.data_ptr() + 2 * 2 * 64
+
+
+def test_not_differentiable_twice():
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention
+
+    q, k, v, table, dout = _tensors(1, 40, 40, 2, 2, 64, 8)
+    out = relative_bias_attention(q, k, v, table, 0.125, max_distance=20)
+    grads = torch.autograd.grad(out, (q, k, v, table), dout, create_graph=True)
+    plain = torch.autograd.grad(relative_bias_attention(q, k, v, table, 0.125, max_distance=20), (q, k, v, table), dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads, plain))
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        grads[0].float().square().sum().backward()
