@@ -30,6 +30,9 @@ __device__ __forceinline__ float bias_log2(float x) {
   const float y = x * kBandLog2e;
   return isinf(x) ? x : fminf(fmaxf(y, -kBiasLimit), kBiasLimit);
 }
+__device__ __forceinline__ __nv_bfloat16* rest_row(const BandArgs& a, int b, int s, int h, int d) {
+  return a.o_rest + ((static_cast<long long>(b) * a.rest_rows + s) * a.Hq + h) * d;
+}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -834,14 +837,26 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = 0;
         }
-        if (row < a.Sq) store_bf16_16(out + c * 16, o, inv);
+        if (row < a.Sq) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+          store_bf16_16(out + c * 16, o, 1.f);
+          if (row < a.rest_rows) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float x = __uint_as_float(o[k]);
+              o[k] = __float_as_uint(x - __bfloat162float(__float2bfloat16(x)));
+            }
+            store_bf16_16(rest_row(a, w.b, row, h, D) + half * (D / 2) + c * 16, o, 1.f);
+          }
+        }
       }
       if (n > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_empty[t]);
       }
-      if (half == 0 && row < a.Sq) {
+      if (half == 0 && row < a.Sq && a.m != nullptr) {
         const long long stat = (static_cast<long long>(w.b) * a.Hq + h) * a.Sq + row;
         a.m[stat] = l > 0.f ? m : INFINITY;  // a row that sees nothing: 2^(x - m) is 0 in the backward pass
         a.l[stat] = l > 0.f ? log2f(l) : 0.f;
@@ -875,10 +890,10 @@ static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
 }
 
 // --------------------------------------------------------------- backward --
-// Two kernels and no atomics: a query tile's dQ and a key tile's dK, dV are each summed by one CTA in a fixed order, at the
+// Two large kernels and no atomics: a query tile's dQ and a key tile's dK, dV are each summed by one CTA in a fixed order, at the
 // price of working the weights out twice (seven products of a tile pair instead of five).
 //
-// Column statistics passed from the first to the second, per (batch, query head, query tile): 128 floats each of
+// Statistics of the query rows that both read, per (batch, query head, query tile): 128 floats each of
 //   c = (far bias - m) - l,  D,  m,  l        (rows behind the last: c = -inf, so that their weights are 0)
 constexpr int kStatBlock = 512;  // floats
 
@@ -922,15 +937,71 @@ struct BandBwdParams {
   int sink_pieces, pieces;
 };
 
-// ---- dQ, D, and the table's gradient ----
+// ---- D and the column statistics ----
+// A block per query tile; D / 8 lanes a row (16 bytes each of dO, O and what was cut off of it), a thread's rows in flight together.
+// In the dQ kernel, a thread per quarter row, the same loads hit a line per lane and cost an item 4000 clocks.
+template <int D>
+__global__ void __launch_bounds__(256) band_stat_kernel(const __grid_constant__ BandBwdParams p) {
+  pdl_enter();
+  const BandArgs& a = p.a;
+  constexpr int kLanes = D == 64 ? 8 : 16;  // 12 of 16 at D = 96
+  constexpr int kRowsAtOnce = 256 / kLanes, kStatRows = 128 / kRowsAtOnce;
+  const int sub = threadIdx.x / kLanes, part = threadIdx.x % kLanes;
+  const long long tile = blockIdx.x;  // (b * Hq + h) * n_qt + qt
+  const int qt = static_cast<int>(tile % p.n_qt), h = static_cast<int>(tile / p.n_qt % a.Hq);
+  const int b = static_cast<int>(tile / p.n_qt / a.Hq);
+  const bool mine = part * 8 < D;
+  uint4 o[kStatRows], rest[kStatRows], g[kStatRows];
+#pragma unroll
+  for (int i = 0; i < kStatRows; ++i) {
+    const int row = qt * 128 + i * kRowsAtOnce + sub;
+    if (mine && row < a.Sq) {
+      o[i] = *reinterpret_cast<const uint4*>(band_row(a.o, a.o_st, b, row, h) + part * 8);
+      rest[i] = row < a.rest_rows ? *reinterpret_cast<const uint4*>(rest_row(a, b, row, h, D) + part * 8) : make_uint4(0, 0, 0, 0);
+      g[i] = *reinterpret_cast<const uint4*>(band_row(a.dout, a.dout_st, b, row, h) + part * 8);
+    } else {
+      o[i] = rest[i] = g[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const float far_bias = a.table == nullptr ? 0.f : bias_log2(table_at(a, h, a.buckets - 1));
+  float* st = p.stat + tile * kStatBlock;
+#pragma unroll
+  for (int i = 0; i < kStatRows; ++i) {
+    const uint32_t ow[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, rw[4] = {rest[i].x, rest[i].y, rest[i].z, rest[i].w};
+    const uint32_t gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = unpack_bf16x2(ow[k]), z = unpack_bf16x2(rw[k]), y = unpack_bf16x2(gw[k]);
+      sum = fmaf(x.x + z.x, y.x, fmaf(x.y + z.y, y.y, sum));
+    }
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const int r = i * kRowsAtOnce + sub, row = qt * 128 + r;
+    if (part == 0) {
+      const long long at = (static_cast<long long>(b) * a.Hq + h) * a.Sq + row;
+      const float m = row < a.Sq ? a.m[at] : INFINITY, l = row < a.Sq ? a.l[at] : 0.f;
+      st[r] = (far_bias - m) - l;
+      st[128 + r] = sum;
+      st[256 + r] = m;
+      st[384 + r] = l;
+    }
+  }
+}
+
+// ---- dQ and the table's gradient ----
 // A CTA works on one query tile: S = Q K^T and dP = dO V^T land in tensor memory, sixteen warps (four threads a row, 32 columns
 // each) turn them into dS, which goes back as the A operand of dQ += dS K.  S and dP of the next tile are computed while
 // dS of this one is.  TMEM: S 0, dP 128, dQ 256, dS (two buffers) from 384.
 //
+// D = dO . O wants O with more bits than a bf16 result has: the error of its rounding is the same for all keys of a row, adds
+// up where terms of dS cancel (few keys: 4.7e-3 of dQ's norm instead of 2.3e-3), and, summed over thousands of keys, is as large
+// as the gradient of the last bucket (1.6e-2 of it).  So a forward pass that will be differentiated also keeps what the rounding
+// cut off, as another bf16 value: of all rows with a bias, else of those that see few keys (the caller says up to which row).
+//
 // dtable: inside tiles that meet distances below t_last the sums along the diagonals (equal distance) are formed by passing a
 // running sum from lane to lane, one row down per column; they are then added by bucket.  All other tiles belong to the last
-// bucket.  Its sum over many keys is small against its terms' rounding: D comes from the output rounded to bf16 and is off by
-// some e, which the rows' sums show (sum_j dS_ij is e times the sum of P, 1, instead of 0); e * P is taken off again.
+// bucket as a whole.
 template <int D>
 struct BandDqSmem {
   static constexpr int kSlabs = (D + 63) / 64;
@@ -942,10 +1013,10 @@ struct BandDqSmem {
   static constexpr int kStages = kStagesK + kStagesV;
   static constexpr int kQ = 0;                     // Q, dO per stage
   static constexpr int kRing = 2 * kQStages * kTile;  // the stages of K, then those of V
-  static constexpr int kBar = kRing + kStages * kTile;
+  static constexpr int kStat = kRing + kStages * kTile;  // per stage of Q
+  static constexpr int kBar = kStat + kQStages * kStatBlock * 4;
   static constexpr int kNumBars = 2 * kStages + 2 * kQStages + 8;
-  static constexpr int kXch = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [2][4][128]
-  static constexpr int kLut = kXch + 4096;                                     // float [entries], the map
+  static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [entries], the map
   // behind them, where the table's gradient is wanted: float bins[16][128], diagonals[16][64]
   static constexpr int kBins = kComputeWarps * (kMaxBuckets + 64) * 4;
   // columns of a row that one of its four threads reads and writes; three do at D = 96
@@ -978,7 +1049,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
   uint64_t* kv_full = bars;                // [SK + SV]
   uint64_t* kv_empty = bars + ST;          // [SK + SV]
   uint64_t* q_full = bars + 2 * ST;        // [QS]
-  uint64_t* q_empty = q_full + QS;         // [QS] last product issued + the warps that read dO
+  uint64_t* q_empty = q_full + QS;         // [QS] last product issued + the warps that read the statistics
   uint64_t* sdp_full = q_empty + QS;
   uint64_t* sdp_read = sdp_full + 1;
   uint64_t* dq_full = sdp_full + 2;
@@ -1060,7 +1131,10 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         const int qs = n_item % QS, use = n_item / QS;
         ++n_item;
         if (use > 0 && !band_wait(&q_empty[qs], (use - 1) & 1, abort_flag, a.status, 81)) break;
-        mbar_expect_tx(&q_full[qs], 2 * L::kTile);
+        const uint32_t stat_bytes = a.table == nullptr ? 1024 : 2048;
+        mbar_expect_tx(&q_full[qs], 2 * L::kTile + stat_bytes);
+        bulk_load(smem + L::kStat + qs * kStatBlock * 4,
+                  p.stat + ((static_cast<long long>(w.b) * a.Hq + w.h) * p.n_qt + w.q0 / 128) * kStatBlock, stat_bytes, &q_full[qs]);
 #pragma unroll
         for (int c = 0; c < NS; ++c) {
           uint8_t* dst = smem + L::kQ + 2 * qs * L::kTile + c * 16384;
@@ -1153,21 +1227,12 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
     const int r = quad * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const bool has_cols = quarter * L::kCols < D;
-    float* xch = reinterpret_cast<float*>(smem + L::kXch);
     float* my_bins = bins + warp * kMaxBuckets;
     float* diag = bins + kComputeWarps * kMaxBuckets + warp * 64;
     const float sl2 = a.scale * kBandLog2e;
     const bool want_table = a.dtable != nullptr;
-    int step = 0, n_item = 0, parity = 0;
+    int step = 0, n_item = 0;
     auto together = [&]() { named_sync(1, kComputeWarps * 32); };
-    // the sum of a row's four values
-    auto row_sum = [&](float mine) {
-      float* x = xch + parity * 512 + r;
-      parity ^= 1;
-      x[quarter * 128] = mine;
-      together();
-      return (x[0] + x[128]) + (x[256] + x[384]);
-    };
     bool ok = true;
     for (int round = 0; round < rounds; ++round) {
       const int item = item_of_round(round);
@@ -1176,55 +1241,26 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
       const int n = w.t.count();
       const int row = w.q0 + r, pos = a.q_pos0 + row, pmin = a.q_pos0 + w.q0;
       const bool valid = row < a.Sq;
-      const long long at_row = (static_cast<long long>(w.b) * a.Hq + w.h) * a.Sq + row;
-      const float m = valid ? a.m[at_row] : INFINITY;
-      const float l = valid ? a.l[at_row] : 0.f;
       float far_bias = 0.f;
       if (a.table != nullptr) {
         together();  // everyone has left the item before
         build_lut(a, w.h, p.t_last, map, lut, threadIdx.x, kComputeWarps * 32);
+        together();
+        far_bias = lut[entries - 1];
       }
-      // D: a quarter of a row of O and dO per thread
-      float dsum = 0.f;
+      float c_far = 0.f, delta = 0.f, m = 0.f, l = 0.f;
       if (n > 0) {
-        constexpr int kChunks = L::kCols / 8;  // of 16 bytes
-        uint4 o[kChunks];
-        if (has_cols) {
-          const uint4* src = reinterpret_cast<const uint4*>(band_row(a.o, a.o_st, w.b, valid ? row : w.q0, w.h)) + quarter * kChunks;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) o[c] = src[c];
-        }
         const int qs = n_item % QS;
         NMB_BAND_WAIT(&q_full[qs], (n_item / QS) & 1, 89);
-        if (has_cols) {
-          const uint8_t* sdo = smem + L::kQ + (2 * qs + 1) * L::kTile;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const int ch = quarter * kChunks + c;
-            const uint4 g = *reinterpret_cast<const uint4*>(sdo + (ch >> 3) * 16384 + swz128_offset(r, ch & 7));
-            const uint32_t ow[4] = {o[c].x, o[c].y, o[c].z, o[c].w}, gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 x = unpack_bf16x2(ow[k]), y = unpack_bf16x2(gw[k]);
-              dsum = fmaf(x.x, y.x, fmaf(x.y, y.y, dsum));
-            }
-          }
-        }
+        const float* st = reinterpret_cast<const float*>(smem + L::kStat) + qs * kStatBlock + r;
+        c_far = st[0];
+        delta = st[128];
+        m = st[256];  // these two are there and used with a table only
+        l = st[384];
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[qs]);
       }
-      dsum = row_sum(dsum);
-      const float delta = valid ? dsum : 0.f;
-      if (a.table != nullptr) far_bias = lut[entries - 1];
-      const float c_far = (far_bias - m) - l;
-      if (quarter == 0) {
-        float* st = p.stat + ((static_cast<long long>(w.b) * a.Hq + w.h) * p.n_qt + w.q0 / 128) * kStatBlock + r;
-        st[0] = c_far;
-        st[128] = delta;
-        st[256] = m;
-        st[384] = l;
-      }
-      float ds_all = 0.f, ds_far = 0.f, p_far = 0.f;
+      float ds_far = 0.f;
       for (int u = 0; u < n; ++u, ++step) {
         const int kv0 = tile_at(w.t, u) * 128, k0 = kv0 + quarter * 32;
         NMB_BAND_WAIT(sdp_full, step & 1, 90);
@@ -1276,18 +1312,14 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(&ds_full[step & 1]);
         if (want_table) {
-          float sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) sum += __uint_as_float(dp[k]);
-          ds_all += sum;
           if (!near) {
-            ds_far += sum;
+            uint64_t sum = pack2(ds_far, 0.f);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) p_far += __uint_as_float(s[k]);
+            for (int k = 0; k < 32; k += 2) sum = add2(sum, pack2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])));
+            float s0, s1;
+            unpack2(sum, s0, s1);
+            ds_far = s0 + s1;
           } else {
-            const int far_to = pos - k0 - p.t_last;  // columns up to this one belong to the last bucket
-#pragma unroll
-            for (int k = 0; k < 32; ++k) p_far += k <= far_to ? __uint_as_float(s[k]) : 0.f;
             // diagonal e holds distance base + e; lane 31 completes one of them per column, the others stay behind at the end
             const int base = pmin + quad * 32 - k0 - 31;
             float run = 0.f;
@@ -1344,9 +1376,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         if (lane == 0) mbar_arrive(dq_empty);
       }
       if (want_table) {
-        const float off = row_sum(ds_all);  // the error of D
-        // what belongs to the last bucket in tiles that were summed by diagonals is in the bins already, and so is its error
-        const float last = warp_sum(ds_far - off * p_far);
+        const float last = warp_sum(ds_far);
         if (lane == 0) my_bins[a.buckets - 1] += last;
         together();
         for (int b = threadIdx.x; b < a.buckets; b += kComputeWarps * 32) {
@@ -1840,7 +1870,7 @@ static int dkv_steps(const BandArgs& a, int tile) {
 // Into how many pieces the steps of a key tile are cut.  Cutting costs the pieces' way through memory and a launch; not
 // cutting leaves SMs idle when there are few key tiles and heads (grouped heads), or when the tiles that hold sinks, which
 // every query sees, take many times as long as the others.  The estimate, in steps: the sum over rounds of the longest item
-// of each, with two steps for an item's beginning and end and two more for a piece.
+// of each, with two steps for an item's beginning and end, one more for a piece and two for the launch that adds them up.
 static void plan_pieces(BandBwdParams& p) {
   const BandArgs& a = p.a;
   const int sms = sm_count(), n_hb = a.Hkv * a.B;
@@ -1855,17 +1885,20 @@ static void plan_pieces(BandBwdParams& p) {
   for (int c : {1, 2, 3, 4, 6, 8, 12, 16}) {
     if (c > longest || (c > 1 && others == 0)) break;
     const int piece = (longest + c - 1) / c;
-    const int cs = p.sink_tiles == 0 ? 1 : std::min(64, (longest_sink + std::max(piece, 4) - 1) / std::max(piece, 4));
-    const long long sink_items = static_cast<long long>(p.sink_tiles) * cs * n_hb, items = sink_items + static_cast<long long>(others) * c * n_hb;
-    double cost = (c > 1 || cs > 1) ? 4.0 : 0.0;
-    for (long long i = 0; i < items; i += sms) {
-      if (i < sink_items) cost += longest_sink / cs + (cs > 1 ? 4 : 2);
-      else cost += (dkv_steps(a, p.sink_tiles + static_cast<int>((i - sink_items) / n_hb / c)) + c - 1) / c + (c > 1 ? 4 : 2);
-    }
-    if (cost < best) {
-      best = cost;
-      p.pieces = c;
-      p.sink_pieces = cs;
+    const int even = p.sink_tiles == 0 ? 1 : std::min(64, (longest_sink + std::max(piece, 4) - 1) / std::max(piece, 4));
+    for (int cs : {1, even}) {
+      const long long sink_items = static_cast<long long>(p.sink_tiles) * cs * n_hb;
+      const long long items = sink_items + static_cast<long long>(others) * c * n_hb;
+      double cost = (c > 1 || cs > 1) ? 2.0 : 0.0;
+      for (long long i = 0; i < items; i += sms) {
+        if (i < sink_items) cost += (longest_sink + cs - 1) / cs + (cs > 1 ? 3 : 2);
+        else cost += (dkv_steps(a, p.sink_tiles + static_cast<int>((i - sink_items) / n_hb / c)) + c - 1) / c + (c > 1 ? 3 : 2);
+      }
+      if (cost < best) {
+        best = cost;
+        p.pieces = c;
+        p.sink_pieces = cs;
+      }
     }
   }
 }
@@ -1893,8 +1926,10 @@ static BandScratch plan_bwd(BandBwdParams& p, const BandArgs& a) {
 template <int D>
 static cudaError_t launch_band_bwd(BandBwdParams& p, long long dq_items, long long dkv_items, bool split, cudaStream_t s) {
   const int lut = p.a.table == nullptr ? 0 : lut_bytes(p.t_last, 1);
+  cudaError_t e = launch_pdl(band_stat_kernel<D>, dim3(static_cast<unsigned>(dq_items)), dim3(256), 0, s, p);
+  if (e != cudaSuccess) return e;
   p.n_items = static_cast<int>(dq_items);
-  cudaError_t e = launch_pdl(band_bwd_dq_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads),
+  e = launch_pdl(band_bwd_dq_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads),
                              BandDqSmem<D>::kLut + lut + (p.a.dtable == nullptr ? 0 : BandDqSmem<D>::kBins), s, p);
   if (e != cudaSuccess) return e;
   p.n_items = static_cast<int>(dkv_items);
@@ -1926,6 +1961,7 @@ static int band_check(const BandArgs* a) {
     return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && t.b * 2 % bytes == 0 && t.s * 2 % bytes == 0 && t.h * 2 % bytes == 0;
   };
   // tile loads want 16 bytes; results are written in pieces of 32
+  if (reinterpret_cast<uintptr_t>(a->o_rest) % 32 != 0) return kBadArgument;
   if (!aligned(a->q, a->q_st, 16) || !aligned(a->k, a->k_st, 16) || !aligned(a->v, a->v_st, 16) || !aligned(a->o, a->o_st, 32) ||
       !aligned(a->dout, a->dout_st, 16) || !aligned(a->dq, a->dq_st, 32) || !aligned(a->dk, a->dk_st, 32) ||
       !aligned(a->dv, a->dv_st, 32))
@@ -2007,6 +2043,6 @@ extern "C" int nmb_band_bwd(const BandArgs* a, void* stream) {
   const cudaError_t e = a->d == 64 ? launch_band_bwd<64>(p, dq_items, dkv_items, split, s)
                       : a->d == 96 ? launch_band_bwd<96>(p, dq_items, dkv_items, split, s)
                                    : launch_band_bwd<128>(p, dq_items, dkv_items, split, s);
-  if (e == cudaSuccess) g_band_launches += 2 + (split || a->dtable != nullptr);
+  if (e == cudaSuccess) g_band_launches += 3 + (split || a->dtable != nullptr);
   return e == cudaSuccess ? 0 : 500 + e;
 }

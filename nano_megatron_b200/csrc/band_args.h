@@ -15,9 +15,10 @@ struct BandStride {
 struct BandArgs {
   const __nv_bfloat16 *q, *k, *v;  // [B, Sq, Hq, d], [B, Skv, Hkv, d]
   __nv_bfloat16* o;
+  __nv_bfloat16* o_rest;  // [B, rest_rows, Hq, d], dense: what rounding cut off of the first rows of o
   const __nv_bfloat16* dout;
   __nv_bfloat16 *dq, *dk, *dv;
-  float* m;           // [B, Hq, Sq]
+  float* m;           // [B, Hq, Sq]; null, as l, for a forward pass without a backward one
   float* l;           // [B, Hq, Sq]
   float* scratch;     // nmb_band_bwd_scratch() floats, backward only
   const void* table;  // [Hq, buckets] bf16 or fp32; null without a bias
@@ -28,7 +29,7 @@ struct BandArgs {
   int B, Hq, Hkv, Sq, Skv, d;
   int q_pos0, window, sinks, buckets;
   float scale;
-  int pad;
+  int rest_rows;
   unsigned short limit[kMaxBuckets];  // first distance of bucket b + 1
 };
 

@@ -72,15 +72,19 @@ void place(T*& ptr, nmb::BandStride& st, const Tensor& t) {
   st = strides(t);
 }
 
-nmb::BandArgs arguments(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& out, const Tensor& stats,
-                        double scale, int64_t window, int64_t sinks, int64_t start, int64_t max_distance) {
+nmb::BandArgs arguments(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& out, const Tensor& rest,
+                        const Tensor& stats, double scale, int64_t window, int64_t sinks, int64_t start, int64_t max_distance) {
   nmb::BandArgs a{};
   place(a.q, a.q_st, q);
   place(a.k, a.k_st, k);
   place(a.v, a.v_st, v);
   place(a.o, a.o_st, out);
-  a.m = stats.data_ptr<float>();
-  a.l = a.m + stats.numel() / 2;
+  if (stats.defined()) {
+    a.o_rest = static_cast<__nv_bfloat16*>(const_cast<void*>(rest.const_data_ptr()));
+    a.rest_rows = static_cast<int>(rest.size(1));
+    a.m = stats.data_ptr<float>();
+    a.l = a.m + stats.numel() / 2;
+  }
   a.B = static_cast<int>(q.size(0));
   a.Sq = static_cast<int>(q.size(1));
   a.Hq = static_cast<int>(q.size(2));
@@ -109,18 +113,31 @@ void* current_stream(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.
 
 struct BandAttention : torch::autograd::Function<BandAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
-                        const std::optional<Tensor>& table_in, double scale, int64_t window, int64_t sinks, int64_t start, int64_t max_distance) {
+                        const std::optional<Tensor>& table_in, double scale, int64_t window, int64_t sinks, int64_t start,
+                        int64_t max_distance, bool train) {
     const c10::cuda::CUDAGuard guard(q_in.device());
     const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
     const Tensor table = table_in.has_value() ? table_in->contiguous() : Tensor();
     const Tensor out = at::empty(q.sizes(), q.options());
-    const Tensor stats = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-    const nmb::BandArgs a = arguments(q, k, v, table, out, stats, scale, window, sinks, start, max_distance);
+    Tensor rest, stats;
+    if (train) {
+      // Rows that see kFewKeys or more do without: there the error of D is below a tenth of the other roundings' (it falls with
+      // the root of their number).  The last bucket's gradient is a sum over all rows, and wants them all.
+      constexpr int64_t kFewKeys = 256;
+      const int64_t rows = q.size(1);
+      const int64_t kept = table.defined() || std::min<int64_t>(window, kFewKeys) + std::min<int64_t>(sinks, kFewKeys) <= kFewKeys
+                               ? rows : std::min(rows, std::max<int64_t>(0, kFewKeys - start));
+      rest = at::empty({q.size(0), kept, q.size(2), q.size(3)}, q.options());
+      stats = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    }
+    const nmb::BandArgs a = arguments(q, k, v, table, out, rest, stats, scale, window, sinks, start, max_distance);
     const int rc = nmb_band_fwd(&a, current_stream(q));
     TORCH_CHECK(rc == 0, "nmb_band_fwd: launcher returned ", rc);
-    ctx->save_for_backward({q, k, v, table, out, stats});
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["numbers"] = std::vector<int64_t>{window, sinks, start, max_distance};
+    if (train) {
+      ctx->save_for_backward({q, k, v, table, out, rest, stats});
+      ctx->saved_data["scale"] = scale;
+      ctx->saved_data["numbers"] = std::vector<int64_t>{window, sinks, start, max_distance};
+    }
     return out;
   }
 
@@ -140,12 +157,12 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
 
   static variable_list gradients(AutogradContext* ctx, const Tensor& dout_in) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &out = saved[4], &stats = saved[5];
-    variable_list result(9);
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &out = saved[4], &rest = saved[5], &stats = saved[6];
+    variable_list result(10);
     const c10::cuda::CUDAGuard guard(q.device());
     const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
     const Tensor dout = dout_in.defined() ? readable(dout_in.is_contiguous() ? dout_in : dout_in.contiguous()) : at::zeros_like(out);
-    nmb::BandArgs a = arguments(q, k, v, table, out, stats, ctx->saved_data["scale"].toDouble(), n[0], n[1], n[2], n[3]);
+    nmb::BandArgs a = arguments(q, k, v, table, out, rest, stats, ctx->saved_data["scale"].toDouble(), n[0], n[1], n[2], n[3]);
     Tensor dq, dk, dv;
     // q, k and v the slices of one packed projection: their gradients go to the slices of one buffer, and are joined
     // without a copy
@@ -185,7 +202,9 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
 
 Tensor band_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& table, double scale, int64_t window,
                       int64_t sinks, int64_t start, int64_t max_distance) {
-  return BandAttention::apply(q, k, v, table, scale, window, sinks, start, max_distance);
+  const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                                    (table.has_value() && table->requires_grad()));
+  return BandAttention::apply(q, k, v, table, scale, window, sinks, start, max_distance, train);
 }
 
 }  // namespace

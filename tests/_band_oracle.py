@@ -60,8 +60,9 @@ def oracle(q, k, v, dout, scale, *, window=None, sinks=0, start=0, table=None, m
     dp = g @ vh.transpose(2, 3)
     delta = (g * out).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    # D comes from the rounded output; dP - D from sums of absolute size |dO| |V| and |dO| |O|
-    soft = (g.abs() * out_bound).sum(-1, keepdim=True) + E * (g.abs() @ vh.abs().transpose(2, 3) + (g * out).abs().sum(-1, keepdim=True))
+    # D comes from the output and what its rounding cut off, both in bf16: an error of the weights' rounding and of U * U;
+    # dP - D from sums of absolute size |dO| |V| and |dO| |O|
+    soft = (g.abs() * (U * U * out.abs() + (U + E) * (p @ vh.abs()))).sum(-1, keepdim=True) + E * (g.abs() @ vh.abs().transpose(2, 3) + (g * out).abs().sum(-1, keepdim=True))
     ds_err = p * soft + E * ds.abs()
 
     def grouped(t):  # sum of a group's query heads

@@ -17,15 +17,16 @@ class _Stride(ctypes.Structure):
 
 
 _TENSORS = ("q", "k", "v", "o", "dout", "dq", "dk", "dv")
+_POINTERS = ("q", "k", "v", "o", "o_rest", "dout", "dq", "dk", "dv", "m", "l", "scratch", "table", "dtable", "status")
 
 
 class _Args(ctypes.Structure):
     """BandArgs of csrc/band_args.h."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in (*_TENSORS, "m", "l", "scratch", "table", "dtable", "status")]
+    _fields_ = ([(n, ctypes.c_void_p) for n in _POINTERS]
                 + [(n + "_st", _Stride) for n in _TENSORS]
                 + [(n, ctypes.c_int) for n in ("table_fp32", "dtable_fp32", "B", "Hq", "Hkv", "Sq", "Skv", "d", "q_pos0", "window",
                                                "sinks", "buckets")]
-                + [("scale", ctypes.c_float), ("pad", ctypes.c_int), ("limit", ctypes.c_ushort * 128)])
+                + [("scale", ctypes.c_float), ("rest_rows", ctypes.c_int), ("limit", ctypes.c_ushort * 128)])
 
 
 def _launches():
@@ -283,7 +284,8 @@ def test_nothing_is_written_outside(sq, skv, d, start, buckets):
     stats = {n: flat(b * hq * sq) for n in ("m", "l")}
     if buckets:
         stats["dtable"] = flat(hq * buckets)
-    args = _Args(B=b, Hq=hq, Hkv=hkv, Sq=sq, Skv=skv, d=d, q_pos0=start, window=50, sinks=3, buckets=buckets, scale=0.125, dtable_fp32=1,
+    rest = torch.full((b * sq * hq * d + 128,), mark, device="cuda", dtype=torch.bfloat16)
+    args = _Args(o_rest=rest[64:].data_ptr(), B=b, Hq=hq, Hkv=hkv, Sq=sq, Skv=skv, d=d, q_pos0=start, window=50, sinks=3, buckets=buckets, scale=0.125, rest_rows=sq, dtable_fp32=1,
                  status=native.status_word(q.device).data_ptr(), table=None if table is None else table.data_ptr())
     if buckets:
         args.limit[:buckets - 1] = ba.relative_bucket_limits(buckets, 128)
@@ -299,6 +301,7 @@ def test_nothing_is_written_outside(sq, skv, d, start, buckets):
     native.check_rc(lib.nmb_band_bwd(ctypes.byref(args), stream), "nmb_band_bwd")
     torch.cuda.synchronize()
     native.check_status()
+    assert (rest[:64] == mark).all() and (rest[-64:] == mark).all() and not (rest[64:-64] == mark).all()
     for n, (big, view) in bufs.items():
         assert (big[:, :pad] == mark).all() and (big[:, pad + view.shape[1]:] == mark).all(), n
         assert not (view == mark).all(), n
