@@ -43,6 +43,26 @@ __device__ __forceinline__ T* band_row(T* ptr, const BandStride& st, int b, int 
   return ptr + b * st.b + s * st.s + h * st.h;
 }
 
+// Division by a number that the launch fixes: multiply by a rounded-up reciprocal and shift (Granlund and Montgomery, 1994).
+// All warps of a CTA work out where their next item lies, and a few divisions each of them cost an item 3000 clocks.
+struct FastDiv {
+  uint32_t mul, shift, d;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t divisor) : d(divisor) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int quot(int n) const {  // 0 <= n < 2^31
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+  __device__ __forceinline__ int quot(int n, int& rest) const {
+    const int q = quot(n);
+    rest = n - q * static_cast<int>(d);
+    return q;
+  }
+};
+
 // ------------------------------------------------------------- key tiles --
 // The tiles of 128 keys that a tile of 128 query rows sees: [0, sink) and [lo, hi].
 struct KeyTiles {
@@ -272,11 +292,24 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// Bounded wait: as mbar_wait, but asleep for up to kNapNs at a time after the first look.  (Even a wait that is satisfied
-// takes about 150 clocks; what a role waits for is ordered so that the awaited thing comes last.)
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait: as mbar_wait, but asleep for up to kNapNs at a time after the first look.  (The first look takes about 50
+// clocks, try_wait 80.)
 constexpr uint32_t kNapNs = 10000;
 __device__ __forceinline__ bool band_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_test_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (true) {
     uint32_t done;
@@ -386,6 +419,7 @@ struct BandFwdParams {
   int s_pad;    // rows of the statistics: n_qt * 128
   int n_items;
   int t_last;   // first distance of the last bucket
+  FastDiv by_hb, by_heads, by_group;  // heads (or pairs of them) times batches; heads (or pairs); query heads of a key head
 };
 
 template <int D>
@@ -410,16 +444,13 @@ struct FwdItem {
 __device__ __forceinline__ FwdItem fwd_item(const BandFwdParams& p, int item) {
   const BandArgs& a = p.a;
   FwdItem w;
-  const int heads = p.pair == 2 ? a.Hq / 2 : a.Hq;
-  const int n_hb = heads * a.B;
-  const int rest = item % n_hb;
+  int rest, h;
   const int tiles = p.pair == 1 ? (p.n_qt + 1) / 2 : p.n_qt;
-  const int tile = tiles - 1 - item / n_hb;
-  w.b = rest / heads;
-  const int h = rest % heads;
+  const int tile = tiles - 1 - p.by_hb.quot(item, rest);
+  w.b = p.by_heads.quot(rest, h);
   w.h[0] = p.pair == 2 ? 2 * h : h;
   w.h[1] = p.pair == 2 ? 2 * h + 1 : h;
-  w.hk = w.h[0] / (a.Hq / a.Hkv);
+  w.hk = p.by_group.quot(w.h[0]);
   w.q0[0] = (p.pair == 1 ? 2 * tile : tile) * 128;
   w.q0[1] = p.pair == 1 ? w.q0[0] + 128 : w.q0[0];
   w.t[0] = key_tiles(a, w.q0[0]);
@@ -499,15 +530,17 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
     report_status(a.status, kBadArgument, 75);
     *abort_flag = 1;
   }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&p.q_map);
+    tma_prefetch_desc(&p.k_map);
+    tma_prefetch_desc(&p.v_map);
+  }
   pdl_enter();  // the set-up above touches no global memory
   if (warp >= kComputeWarps) {
     NMB_BAND_FEW_REGISTERS;
     if (warp == kLoadWarp) {
     // ------------------------------------------------------------ producer --
     if (lane == 0) {
-      tma_prefetch_desc(&p.q_map);
-      tma_prefetch_desc(&p.k_map);
-      tma_prefetch_desc(&p.v_map);
       int pos = 0, n_q[2] = {0, 0};
       bool ok = true;
       for (int round = 0; ok; ++round) {
@@ -935,6 +968,8 @@ struct BandBwdParams {
   int t_last;
   int sink_tiles;   // dK, dV: key tiles that hold sinks, their pieces, the pieces of the others
   int sink_pieces, pieces;
+  FastDiv by_hqb, by_hq, by_group;                        // dQ: query heads times batches, query heads; query heads of a key head
+  FastDiv by_hkvb, by_hkv, by_sink_pieces, by_pieces;     // dK, dV: the same of key heads, and the pieces
 };
 
 // ---- D and the column statistics ----
@@ -989,10 +1024,23 @@ __global__ void __launch_bounds__(256) band_stat_kernel(const __grid_constant__ 
   }
 }
 
+// The sixteen compute warps of the two kernels below work as one group on a tile of 128 x 128 weights, or (D = 64) as two
+// groups on one half of its columns each, with tensor-memory columns, accumulators, barriers and an issuer of their own: while
+// one group works out weights (16 exponentials a clock and SM: 512 clocks for its half) the other waits, loads and stores.  At
+// D > 64 there are no columns for a second set of accumulators, and products with half the columns would take longer than the
+// weights (59 clocks instead of 34 for a 128 x 64 x 16 product out of shared memory).
+template <int D>
+struct BandGroups {
+  static constexpr int kGroups = D == 64 ? 2 : 1;
+  static constexpr int kWidth = 128 / kGroups;               // columns of a group
+  static constexpr int kWarps = kComputeWarps / kGroups;
+  static constexpr int kQuarters = 4 / kGroups;              // of 32 columns, a thread's share of a row
+};
+
 // ---- dQ and the table's gradient ----
 // A CTA works on one query tile: S = Q K^T and dP = dO V^T land in tensor memory, sixteen warps (four threads a row, 32 columns
 // each) turn them into dS, which goes back as the A operand of dQ += dS K.  S and dP of the next tile are computed while
-// dS of this one is.  TMEM: S 0, dP 128, dQ 256, dS (two buffers) from 384.
+// dS of this one is.  TMEM: S 0, dP 128, dQ 256 (a second one for the second group at 256 + D), dS (two buffers) from 384.
 //
 // D = dO . O wants O with more bits than a bf16 result has: the error of its rounding is the same for all keys of a row, adds
 // up where terms of dS cancel (few keys: 4.7e-3 of dQ's norm instead of 2.3e-3), and, summed over thousands of keys, is as large
@@ -1015,7 +1063,7 @@ struct BandDqSmem {
   static constexpr int kRing = 2 * kQStages * kTile;  // the stages of K, then those of V
   static constexpr int kStat = kRing + kStages * kTile;  // per stage of Q
   static constexpr int kBar = kStat + kQStages * kStatBlock * 4;
-  static constexpr int kNumBars = 2 * kStages + 2 * kQStages + 8;
+  static constexpr int kNumBars = 2 * kStages + 2 * kQStages + 11;
   static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [entries], the map
   // behind them, where the table's gradient is wanted: float bins[16][128], diagonals[16][64]
   static constexpr int kBins = kComputeWarps * (kMaxBuckets + 64) * 4;
@@ -1031,11 +1079,10 @@ struct DqItem {
 __device__ __forceinline__ DqItem dq_item(const BandBwdParams& p, int item) {
   const BandArgs& a = p.a;
   DqItem w;
-  const int n_hb = a.Hq * a.B;
-  w.h = item % n_hb % a.Hq;
-  w.b = item % n_hb / a.Hq;
-  w.hk = w.h / (a.Hq / a.Hkv);
-  w.q0 = (p.n_qt - 1 - item / n_hb) * 128;
+  int rest;
+  w.q0 = (p.n_qt - 1 - p.by_hqb.quot(item, rest)) * 128;
+  w.b = p.by_hq.quot(rest, w.h);
+  w.hk = p.by_group.quot(w.h);
   w.t = key_tiles(a, w.q0);
   return w;
 }
@@ -1043,20 +1090,20 @@ __device__ __forceinline__ DqItem dq_item(const BandBwdParams& p, int item) {
 template <int D>
 __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __grid_constant__ BandBwdParams p) {
   using L = BandDqSmem<D>;
+  using G = BandGroups<D>;
   constexpr int NS = L::kSlabs, ST = L::kStages, SK = L::kStagesK, SV = L::kStagesV, QS = L::kQStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* kv_full = bars;                // [SK + SV]
   uint64_t* kv_empty = bars + ST;          // [SK + SV]
   uint64_t* q_full = bars + 2 * ST;        // [QS]
-  uint64_t* q_empty = q_full + QS;         // [QS] last product issued + the warps that read the statistics
-  uint64_t* sdp_full = q_empty + QS;
-  uint64_t* sdp_read = sdp_full + 1;
-  uint64_t* dq_full = sdp_full + 2;
-  uint64_t* dq_empty = sdp_full + 3;
-  // one for even and one for odd steps, as the buffers of dS: with one, a step could be over twice before it was looked at
-  uint64_t* ds_full = sdp_full + 4;      // [2]
-  uint64_t* step_done = sdp_full + 6;    // [2] dQ += dS K of a step
+  uint64_t* q_empty = q_full + QS;         // [QS] the issuers + the warps that read the statistics
+  uint64_t* sdp_full = q_empty + QS;       // [groups], as all that follow
+  uint64_t* sdp_read = sdp_full + 2;
+  uint64_t* dq_full = sdp_full + 4;
+  uint64_t* ds_full = sdp_full + 6;        // [groups][2]: one for even and one for odd steps, as the buffers of dS (with one, a
+                                           // step could be over twice before it was looked at)
+  uint64_t* dq_empty = sdp_full + 10;      // one for both
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const BandArgs& a = p.a;
@@ -1074,19 +1121,19 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], G::kGroups);  // the issuers
     }
     for (int s = 0; s < QS; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 1 + kComputeWarps);
+      mbar_init(&q_empty[s], G::kGroups + kComputeWarps);
     }
-    mbar_init(sdp_full, 1);
-    mbar_init(sdp_read, kComputeWarps);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&ds_full[s], kComputeWarps);
-      mbar_init(&step_done[s], 1);
+    for (int g = 0; g < G::kGroups; ++g) {
+      mbar_init(&sdp_full[g], 1);
+      mbar_init(&sdp_read[g], G::kWarps);
+      mbar_init(&dq_full[g], 1);
+      mbar_init(&ds_full[2 * g], G::kWarps);
+      mbar_init(&ds_full[2 * g + 1], G::kWarps);
     }
-    mbar_init(dq_full, 1);
     mbar_init(dq_empty, kComputeWarps);
     *abort_flag = 0;
     fence_mbar_init();
@@ -1109,6 +1156,12 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
     report_status(a.status, kBadArgument, 75);
     *abort_flag = 1;
   }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&p.q_map);
+    tma_prefetch_desc(&p.k_map);
+    tma_prefetch_desc(&p.v_map);
+    tma_prefetch_desc(&p.do_map);
+  }
   pdl_enter();
   const int rounds = (p.n_items + gridDim.x - 1) / gridDim.x;
 
@@ -1116,10 +1169,6 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
     NMB_BAND_FEW_REGISTERS;
     if (warp == kLoadWarp && lane == 0) {
       // ---------------------------------------------------------- producer --
-      tma_prefetch_desc(&p.q_map);
-      tma_prefetch_desc(&p.do_map);
-      tma_prefetch_desc(&p.k_map);
-      tma_prefetch_desc(&p.v_map);
       int pos = 0, n_item = 0;
       bool ok = true;
       for (int round = 0; round < rounds && ok; ++round) {
@@ -1154,13 +1203,33 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
           ok = load(&p.k_map, pos % SK, pos / SK, j) && load(&p.v_map, SK + pos % SV, pos / SV, j);
         }
       }
-    } else if (warp == kMmaWarp) {
-      // ---------------------------------------------- MMA issuer: S and dP --
-      constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
-      const uint32_t ring = smem_u32(smem + L::kRing);
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + G::kGroups) {
+      // -------------------------------------------------------- MMA issuer --
+      // In order: S and dP of a step once those of the step before have been read, then dQ of the step before.  Whoever sees S
+      // and dP of a step therefore knows that dQ of the step before the last has been added, whose dS buffer is next.
+      constexpr uint32_t idesc_s = make_idesc_bf16(128, G::kWidth, false, false);
+      constexpr uint32_t idesc_dq = make_idesc_bf16(128, D, false, true);
+      const int g = warp - kMmaWarp;
+      const uint32_t ring = smem_u32(smem + L::kRing) + g * G::kWidth * 128;  // this group's rows of K and V
+      const uint32_t t_s = tmem + g * G::kWidth, t_dq = tmem + kDq + g * D, t_ds = tmem + kDs + g * (G::kWidth / 2);
       const bool one = elect_one();
       uint32_t step = 0, n_item = 0;  // tiles and items begun
+      bool prev_first = false, prev_last = false;
+      uint32_t prev_item = 0;
       bool ok = true;
+      // dQ += dS K of step s
+      auto issue_dq = [&](uint32_t s, bool first, bool last, uint32_t item_no) {
+        if (first && item_no > 0 && !band_wait(dq_empty, (item_no - 1) & 1, abort_flag, a.status, 83)) return false;
+        if (!band_wait(&ds_full[2 * g + (s & 1)], (s >> 1) & 1, abort_flag, a.status, 84)) return false;
+        tc_fence_after();
+        const uint32_t st = s % SK;
+        if (one) {
+          mma_apply<G::kWidth / 16, 8, 0>(t_dq, t_ds + (s & 1) * 64, desc_mn(ring + st * L::kTile), idesc_dq, first);
+          tc_commit(&kv_empty[st]);
+          if (last) tc_commit(&dq_full[g]);
+        }
+        return true;
+      };
       for (int round = 0; round < rounds && ok; ++round) {
         const int item = item_of_round(round);
         if (item >= p.n_items) continue;
@@ -1171,54 +1240,31 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         const uint32_t q_low = desc_k(smem_u32(smem + L::kQ + 2 * qs * L::kTile));
         for (int u = 0; u < n; ++u, ++step) {
           const uint32_t sk = step % SK, sv = SK + step % SV;
-          // the buffer of dS that this step's scores will fill was last read two steps ago; done before they are is done
-          // before anyone writes to it
-          ok = (u > 0 || band_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 85)) &&
-               band_wait(&kv_full[sk], (step / SK) & 1, abort_flag, a.status, 86) &&
-               (step < 2 || band_wait(&step_done[step & 1], ((step - 2) >> 1) & 1, abort_flag, a.status, 83)) &&
-               (step == 0 || band_wait(sdp_read, (step - 1) & 1, abort_flag, a.status, 88));
+          const BandBar k_bar{&kv_full[sk], (step / SK) & 1}, v_bar{&kv_full[sv], (step / SV) & 1};
+          ok = u > 0 || band_wait(&q_full[qs], (n_item / QS) & 1, abort_flag, a.status, 85);
+          if (!ok) break;
+          ok = step == 0 ? band_wait(k_bar.bar, k_bar.parity, abort_flag, a.status, 86)
+                         : band_wait_all(abort_flag, a.status, 88, k_bar, BandBar{&sdp_read[g], (step - 1) & 1});
           if (!ok) break;
           tc_fence_after();
-          if (one) mma_scores<D>(tmem, q_low, desc_k(ring + sk * L::kTile), idesc_s);
-          ok = band_wait(&kv_full[sv], (step / SV) & 1, abort_flag, a.status, 87);
+          if (one) mma_scores<D>(t_s, q_low, desc_k(ring + sk * L::kTile), idesc_s);
+          ok = band_wait(v_bar.bar, v_bar.parity, abort_flag, a.status, 87);
           if (!ok) break;
           if (one) {
-            mma_scores<D>(tmem + kDp, q_low + (L::kTile >> 4), desc_k(ring + sv * L::kTile), idesc_s);
-            tc_commit(sdp_full);
+            mma_scores<D>(t_s + kDp, q_low + (L::kTile >> 4), desc_k(ring + sv * L::kTile), idesc_s);
+            tc_commit(&sdp_full[g]);
             tc_commit(&kv_empty[sv]);
             if (u == n - 1) tc_commit(&q_empty[qs]);
           }
-        }
-        ++n_item;
-      }
-    } else if (warp == kMmaWarp + 1) {
-      // ----------------------------------------------------- MMA issuer: dQ --
-      constexpr uint32_t idesc_dq = make_idesc_bf16(128, D, false, true);
-      const uint32_t ring = smem_u32(smem + L::kRing);
-      const bool one = elect_one();
-      uint32_t step = 0, n_item = 0;
-      bool ok = true;
-      for (int round = 0; round < rounds && ok; ++round) {
-        const int item = item_of_round(round);
-        if (item >= p.n_items) continue;
-        const int n = dq_item(p, item).t.count();
-        if (n == 0) continue;
-        for (int u = 0; u < n; ++u, ++step) {
-          const uint32_t sk = step % SK;
-          ok = band_wait(&kv_full[sk], (step / SK) & 1, abort_flag, a.status, 93) &&
-               (u > 0 || n_item == 0 || band_wait(dq_empty, (n_item - 1) & 1, abort_flag, a.status, 94)) &&
-               band_wait(&ds_full[step & 1], (step >> 1) & 1, abort_flag, a.status, 84);
+          if (step > 0) ok = issue_dq(step - 1, prev_first, prev_last, prev_item);
           if (!ok) break;
-          tc_fence_after();
-          if (one) {
-            mma_apply<8, 8, 0>(tmem + kDq, tmem + kDs + (step & 1) * 64, desc_mn(ring + sk * L::kTile), idesc_dq, u == 0);
-            tc_commit(&step_done[step & 1]);
-            tc_commit(&kv_empty[sk]);
-            if (u == n - 1) tc_commit(dq_full);
-          }
+          prev_first = u == 0;
+          prev_last = u == n - 1;
+          prev_item = n_item;
         }
         ++n_item;
       }
+      if (ok && step > 0) issue_dq(step - 1, prev_first, prev_last, prev_item);
     }
   } else {
     NMB_BAND_MORE_REGISTERS;
@@ -1226,6 +1272,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
     const int quad = warp & 3, quarter = warp >> 2;
     const int r = quad * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const int g = quarter / G::kQuarters;
     const bool has_cols = quarter * L::kCols < D;
     float* my_bins = bins + warp * kMaxBuckets;
     float* diag = bins + kComputeWarps * kMaxBuckets + warp * 64;
@@ -1263,7 +1310,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
       float ds_far = 0.f;
       for (int u = 0; u < n; ++u, ++step) {
         const int kv0 = tile_at(w.t, u) * 128, k0 = kv0 + quarter * 32;
-        NMB_BAND_WAIT(sdp_full, step & 1, 90);
+        NMB_BAND_WAIT(&sdp_full[g], step & 1, 90);
         tc_fence_after();
         uint32_t s[32], dp[32];
         tmem_ld_32x32(t_row + quarter * 32, s);
@@ -1271,7 +1318,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(sdp_read);
+        if (lane == 0) mbar_arrive(&sdp_read[g]);
         const bool near = a.table != nullptr && pmin - (kv0 + 127) < p.t_last;
         const bool added = near || (a.table != nullptr && fabsf(far_bias) > 1e30f);
         const bool whole = kv0 + 127 <= pmin && kv0 + 127 < a.Skv && (pmin + 127 - kv0 < a.window || kv0 + 127 < a.sinks);
@@ -1310,7 +1357,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ds_full[step & 1]);
+        if (lane == 0) mbar_arrive(&ds_full[2 * g + (step & 1)]);
         if (want_table) {
           if (!near) {
             uint64_t sum = pack2(ds_far, 0.f);
@@ -1351,7 +1398,8 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         }
       }
       if (n > 0) {
-        NMB_BAND_WAIT(dq_full, n_item & 1, 91);
+        NMB_BAND_WAIT(&dq_full[0], n_item & 1, 91);
+        if (G::kGroups == 2) NMB_BAND_WAIT(&dq_full[1], n_item & 1, 91);
         ++n_item;
         tc_fence_after();
       }
@@ -1362,7 +1410,15 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
           uint32_t v[16];
           if (n > 0) {
             tmem_ld_32x16(t_row + kDq + quarter * L::kCols + c * 16, v);
-            tmem_ld_wait();
+            if (G::kGroups == 2) {
+              uint32_t v2[16];
+              tmem_ld_32x16(t_row + kDq + D + quarter * L::kCols + c * 16, v2);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __uint_as_float(v2[k]));
+            } else {
+              tmem_ld_wait();
+            }
           } else {
 #pragma unroll
             for (int k = 0; k < 16; ++k) v[k] = 0;
@@ -1407,18 +1463,19 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
 // ---- dK and dV ----
 // A CTA works on one key tile of one key head, over the query heads of the group and the query tiles that see it, or on a
 // piece of them.  S^T = K Q^T and dP^T = V dO^T have keys as rows, so P^T and dS^T go straight back to tensor memory as A
-// operands of dV += P^T dO and dK += dS^T Q.  TMEM: S^T 0, dP^T 128, dV 256, dK 256 + D; with D = 64 P^T and dS^T have
-// columns of their own (384, 448), else they overwrite S^T and dP^T.
+// operands of dV += P^T dO and dK += dS^T Q; they overwrite what they came from, each thread its own columns.  TMEM: S^T 0,
+// dP^T 128, dV 256, dK 256 + D; those of the second group at 384.
 template <int D>
 struct BandDkvSmem {
   static constexpr int kSlabs = (D + 63) / 64;
   static constexpr int kTile = kSlabs * 16384;
-  static constexpr int kStages = D == 64 ? 4 : 2;  // Q, dO and the column statistics
-  static constexpr int kK = 0;                     // K, V
-  static constexpr int kRing = 2 * kTile;
+  static constexpr int kStages = D == 64 ? 3 : 2;    // Q, dO and the column statistics
+  static constexpr int kKvStages = D == 64 ? 2 : 1;  // K, V
+  static constexpr int kK = 0;
+  static constexpr int kRing = 2 * kKvStages * kTile;
   static constexpr int kStat = kRing + 2 * kStages * kTile;
   static constexpr int kBar = kStat + kStages * kStatBlock * 4;
-  static constexpr int kNumBars = 2 * kStages + 9;
+  static constexpr int kNumBars = 2 * kStages + 2 * kKvStages + 11;
   static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;
   static constexpr int kCols = D == 96 ? 32 : D / 4;  // as in the dQ kernel
 };
@@ -1432,32 +1489,23 @@ struct DkvItem {
 __device__ __forceinline__ DkvItem dkv_item(const BandBwdParams& p, int item) {
   const BandArgs& a = p.a;
   DkvItem w;
-  const int n_hb = a.Hkv * a.B;
-  const int sink_items = p.sink_tiles * p.sink_pieces * n_hb;
-  int tile, piece, pieces;
-  if (item < sink_items) {
-    pieces = p.sink_pieces;
-    w.slot = item;
-    tile = item / n_hb / pieces;
-    piece = item / n_hb % pieces;
-  } else {
-    pieces = p.pieces;
-    const int rest = item - sink_items;
-    w.slot = (p.sink_pieces > 1 ? sink_items : 0) + rest;
-    tile = p.sink_tiles + rest / n_hb / pieces;
-    piece = rest / n_hb % pieces;
-  }
-  if (pieces == 1) w.slot = -1;
-  w.hk = item % n_hb % a.Hkv;
-  w.b = item % n_hb / a.Hkv;
+  const int sink_items = p.sink_tiles * p.sink_pieces * a.Hkv * a.B;
+  const bool sink = item < sink_items;
+  const int rank = sink ? item : item - sink_items, pieces = sink ? p.sink_pieces : p.pieces;
+  int hb, piece;
+  const int at = p.by_hkvb.quot(rank, hb);
+  const int tile = (sink ? 0 : p.sink_tiles) + (sink ? p.by_sink_pieces : p.by_pieces).quot(at, piece);
+  w.slot = pieces == 1 ? -1 : sink ? rank : (p.sink_pieces > 1 ? sink_items : 0) + rank;
+  w.b = p.by_hkv.quot(hb, w.hk);
   w.kv0 = tile * 128;
   const int first = max(0, w.kv0 - a.q_pos0);
   const int last = w.kv0 < a.sinks ? a.Sq - 1 : min(a.Sq - 1, min(w.kv0 + 127, a.Skv - 1) - a.q_pos0 + a.window - 1);
   w.first_qt = first >> 7;
   w.per_head = first <= last ? (last >> 7) - w.first_qt + 1 : 0;
-  const int n = w.per_head * (a.Hq / a.Hkv);
-  w.from = static_cast<int>(static_cast<long long>(n) * piece / pieces);
-  w.to = static_cast<int>(static_cast<long long>(n) * (piece + 1) / pieces);
+  const int n = w.per_head * static_cast<int>(p.by_group.d);
+  const int len = (sink ? p.by_sink_pieces : p.by_pieces).quot(n + pieces - 1);
+  w.from = min(n, piece * len);
+  w.to = min(n, w.from + len);
   return w;
 }
 
@@ -1487,23 +1535,21 @@ struct DkvWalk {
 template <int D>
 __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __grid_constant__ BandBwdParams p) {
   using L = BandDkvSmem<D>;
-  constexpr int NS = L::kSlabs, ST = L::kStages;
-  constexpr bool kOwn = D == 64;  // P^T and dS^T have their own columns
-  constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D, kP = kOwn ? 384 : 0, kDs = kOwn ? 448 : 128;
-  constexpr int kQuarter = kOwn ? 16 : 32;  // a warp that is ahead must not write over what another still reads
+  using G = BandGroups<D>;
+  constexpr int NS = L::kSlabs, ST = L::kStages, KS = L::kKvStages;
+  constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* q_full = bars;             // [ST]
-  uint64_t* q_empty = bars + ST;       // [ST] both issuers + the warps that read the statistics
-  uint64_t* kv_full = bars + 2 * ST;
-  uint64_t* kv_empty = kv_full + 1;    // both issuers, as for acc_full
-  uint64_t* s_full = kv_full + 2;
-  uint64_t* s_read = kv_full + 3;
-  uint64_t* dp_full = kv_full + 4;
-  uint64_t* p_full = kv_full + 5;
-  uint64_t* ds_full = kv_full + 6;
-  uint64_t* acc_full = kv_full + 7;
-  uint64_t* acc_empty = kv_full + 8;
+  uint64_t* q_full = bars;              // [ST]
+  uint64_t* q_empty = bars + ST;        // [ST] the issuers + the warps that read the statistics
+  uint64_t* kv_full = bars + 2 * ST;    // [KS]
+  uint64_t* kv_empty = kv_full + KS;    // [KS] the issuers
+  uint64_t* s_full = kv_empty + KS;     // [groups], as all that follow
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* p_full = s_full + 4;
+  uint64_t* ds_full = s_full + 6;
+  uint64_t* acc_full = s_full + 8;
+  uint64_t* acc_empty = s_full + 10;    // one for both
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const BandArgs& a = p.a;
@@ -1519,16 +1565,19 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 2 + kComputeWarps);
+      mbar_init(&q_empty[s], G::kGroups + kComputeWarps);
     }
-    mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 2);
-    mbar_init(s_full, 1);
-    mbar_init(s_read, kComputeWarps);
-    mbar_init(dp_full, 1);
-    mbar_init(p_full, kComputeWarps);
-    mbar_init(ds_full, kComputeWarps);
-    mbar_init(acc_full, kOwn ? 1 : 2);
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], G::kGroups);
+    }
+    for (int g = 0; g < G::kGroups; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&dp_full[g], 1);
+      mbar_init(&p_full[g], G::kWarps);
+      mbar_init(&ds_full[g], G::kWarps);
+      mbar_init(&acc_full[g], 1);
+    }
     mbar_init(acc_empty, kComputeWarps);
     *abort_flag = 0;
     fence_mbar_init();
@@ -1547,29 +1596,33 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
     report_status(a.status, kBadArgument, 75);
     *abort_flag = 1;
   }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&p.q_map);
+    tma_prefetch_desc(&p.k_map);
+    tma_prefetch_desc(&p.v_map);
+    tma_prefetch_desc(&p.do_map);
+  }
   pdl_enter();
-  const int group = a.Hq / a.Hkv;
+  const int group = static_cast<int>(p.by_group.d);
 
   if (warp >= kComputeWarps) {
     NMB_BAND_FEW_REGISTERS;
     if (warp == kLoadWarp && lane == 0) {
       // ---------------------------------------------------------- producer --
-      tma_prefetch_desc(&p.q_map);
-      tma_prefetch_desc(&p.do_map);
-      tma_prefetch_desc(&p.k_map);
-      tma_prefetch_desc(&p.v_map);
       const uint32_t stat_bytes = a.table == nullptr ? 1024 : 2048;
       DkvWalk x;
       int n = 0, n_item = 0;
       for (bool more = x.open(p, 0); more; more = x.next(p), ++n) {
         if (x.first()) {
-          if (n_item > 0 && !band_wait(kv_empty, (n_item - 1) & 1, abort_flag, a.status, 101)) break;
+          const int ks = n_item % KS, kuse = n_item / KS;
+          if (kuse > 0 && !band_wait(&kv_empty[ks], (kuse - 1) & 1, abort_flag, a.status, 101)) break;
           ++n_item;
-          mbar_expect_tx(kv_full, 2 * L::kTile);
+          mbar_expect_tx(&kv_full[ks], 2 * L::kTile);
 #pragma unroll
           for (int c = 0; c < NS; ++c) {
-            tma_load_4d(smem + L::kK + c * 16384, &p.k_map, kv_full, c * 64, x.w.kv0, x.w.hk, x.w.b);
-            tma_load_4d(smem + L::kK + L::kTile + c * 16384, &p.v_map, kv_full, c * 64, x.w.kv0, x.w.hk, x.w.b);
+            uint8_t* dst = smem + L::kK + 2 * ks * L::kTile + c * 16384;
+            tma_load_4d(dst, &p.k_map, &kv_full[ks], c * 64, x.w.kv0, x.w.hk, x.w.b);
+            tma_load_4d(dst + L::kTile, &p.v_map, &kv_full[ks], c * 64, x.w.kv0, x.w.hk, x.w.b);
           }
         }
         const int st = n % ST, use = n / ST;
@@ -1585,68 +1638,63 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
         bulk_load(smem + L::kStat + st * kStatBlock * 4,
                   p.stat + ((static_cast<long long>(x.w.b) * a.Hq + h) * p.n_qt + qt) * kStatBlock, stat_bytes, &q_full[st]);
       }
-    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
-      // ------------------------------------------------------- MMA issuers --
-      // Columns that are written by one product and read by another as operand stay with one issuer, whose products run in
-      // order: S^T and, where P^T overwrites it, dV with the first; dP^T and dK (and else dV) with the second.  So dP^T of a
-      // step is complete after dK (and dV) of the step before, and S^T after dV of the step before where that matters.
-      constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + G::kGroups) {
+      // -------------------------------------------------------- MMA issuer --
+      // In order, for step n: dV with P^T, then S^T of the next step in its place; dK with dS^T, then dP^T of the next step.
+      // The tensor core has the products of one operand to work on while the compute warps make the other.
+      constexpr uint32_t idesc_s = make_idesc_bf16(128, G::kWidth, false, false);
       constexpr uint32_t idesc_d = make_idesc_bf16(128, D, false, true);
-      const uint32_t sk = smem_u32(smem + L::kK), ring = smem_u32(smem + L::kRing);
+      const int g = warp - kMmaWarp;
+      const uint32_t kv = smem_u32(smem + L::kK), ring = smem_u32(smem + L::kRing) + g * G::kWidth * 128;  // this group's queries
+      const uint32_t t_s = tmem + g * G::kWidth, t_dv = tmem + kDv + g * 128, t_dk = tmem + kDk + g * 128;
       const bool one = elect_one();
-      const bool is_s = warp == kMmaWarp;
-      const uint32_t a_low = desc_k(is_s ? sk : sk + L::kTile), d = is_s ? tmem : tmem + kDp, b_off = is_s ? 0 : L::kTile;
       DkvWalk x;
       uint32_t n = 0, n_item = 0;  // step, item of `x`
       bool more = x.open(p, 0);
-      // S^T or dP^T of a step
-      auto scores = [&](uint32_t n, bool last) {
-        tc_fence_after();
+      auto q_bar = [&](uint32_t i) { return BandBar{&q_full[i % ST], (i / ST) & 1}; };
+      auto scores = [&](uint32_t i, uint32_t item) {
         if (one) {
-          mma_scores<D>(d, a_low, desc_k(ring + 2 * (n % ST) * L::kTile + b_off), idesc_s);
-          tc_commit(is_s ? s_full : dp_full);
-          if (last) tc_commit(kv_empty);
+          mma_scores<D>(t_s, desc_k(kv + 2 * (item % KS) * L::kTile), desc_k(ring + 2 * (i % ST) * L::kTile), idesc_s);
+          tc_commit(&s_full[g]);
         }
       };
-      bool ok = more && band_wait(kv_full, 0, abort_flag, a.status, 103) && band_wait(&q_full[0], 0, abort_flag, a.status, 104);
-      if (ok) scores(0, x.last());
+      auto dps = [&](uint32_t i, uint32_t item, bool last) {
+        if (one) {
+          mma_scores<D>(t_s + kDp, desc_k(kv + (2 * (item % KS) + 1) * L::kTile), desc_k(ring + (2 * (i % ST) + 1) * L::kTile), idesc_s);
+          tc_commit(&dp_full[g]);
+          if (last) tc_commit(&kv_empty[item % KS]);
+        }
+      };
+      bool ok = more && band_wait_all(abort_flag, a.status, 103, BandBar{&kv_full[0], 0}, q_bar(0));
+      if (ok) {
+        tc_fence_after();
+        scores(0, 0);
+        dps(0, 0, x.last());
+      }
       while (ok && more) {
         DkvWalk y = x;
         const bool ahead = y.next(p), fresh = ahead && y.first(), y_last = ahead && y.last();
         const bool x_first = x.first(), x_last = x.last();
         const uint32_t n_item2 = n_item + fresh, sq = ring + 2 * (n % ST) * L::kTile;
-        // what the next step's scores need; looked for while the products of this step run
-        auto next_there = [&]() {
-          return (!fresh || band_wait(kv_full, n_item2 & 1, abort_flag, a.status, 105)) &&
-                 band_wait(&q_full[(n + 1) % ST], ((n + 1) / ST) & 1, abort_flag, a.status, 106);
-        };
-        if (kOwn && is_s) {
-          if (ahead) {
-            if (!next_there() || !band_wait(s_read, n & 1, abort_flag, a.status, 107)) break;
-            scores(n + 1, y_last);
-          }
-          if (one) tc_commit(&q_empty[n % ST]);
-        } else {
-          if (x_first && n_item > 0 && !band_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
-          if (kOwn || is_s) {
-            if (!band_wait(p_full, n & 1, abort_flag, a.status, 109)) break;
-            tc_fence_after();
-            if (one) mma_apply<8, 2, kQuarter>(tmem + kDv, tmem + kP, desc_mn(sq + L::kTile), idesc_d, x_first);
-          }
-          if (!is_s) {
-            if (!band_wait(ds_full, n & 1, abort_flag, a.status, 111)) break;
-            tc_fence_after();
-            if (one) mma_apply<8, 2, kQuarter>(tmem + kDk, tmem + kDs, desc_mn(sq), idesc_d, x_first);
-          }
-          if (one) {
-            tc_commit(&q_empty[n % ST]);
-            if (x_last) tc_commit(acc_full);
-          }
-          if (ahead) {
-            if (!next_there()) break;
-            scores(n + 1, y_last);
-          }
+        if (x_first && n_item > 0 && !band_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
+        if (!band_wait(&p_full[g], n & 1, abort_flag, a.status, 109)) break;
+        tc_fence_after();
+        if (one) mma_apply<G::kWidth / 16, 2, 32>(t_dv, t_s, desc_mn(sq + L::kTile), idesc_d, x_first);
+        if (ahead) {  // looked for while dV runs
+          const BandBar k_bar{&kv_full[n_item2 % KS], (n_item2 / KS) & 1};
+          ok = fresh ? band_wait_all(abort_flag, a.status, 106, k_bar, q_bar(n + 1))
+                     : band_wait(q_bar(n + 1).bar, q_bar(n + 1).parity, abort_flag, a.status, 106);
+          if (!ok) break;
+          scores(n + 1, n_item2);
         }
+        if (!band_wait(&ds_full[g], n & 1, abort_flag, a.status, 111)) break;
+        tc_fence_after();
+        if (one) {
+          mma_apply<G::kWidth / 16, 2, 32>(t_dk, t_s + kDp, desc_mn(sq), idesc_d, x_first);
+          tc_commit(&q_empty[n % ST]);
+          if (x_last) tc_commit(&acc_full[g]);
+        }
+        if (ahead) dps(n + 1, n_item2, y_last);
         x = y;
         more = ahead;
         n_item = n_item2;
@@ -1659,6 +1707,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
     const int quad = warp & 3, quarter = warp >> 2;
     const int r = quad * 32 + lane;  // key of the tile == TMEM lane
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const int g = quarter / G::kQuarters;
     const bool has_cols = quarter * L::kCols < D;
     const float sl2 = a.scale * kBandLog2e;
     const int rounds = (p.n_items + gridDim.x - 1) / gridDim.x;
@@ -1672,8 +1721,13 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
       const int j = w.kv0 + r;
       int lut_h = -1;
       float far_bias = 0.f;
+      const int per_head = max(w.per_head, 1);
+      int h = w.hk * group + w.from / per_head, qt = w.first_qt + w.from % per_head - 1;
       for (int step = w.from; step < w.to; ++step, ++n) {
-        const int h = w.hk * group + step / w.per_head, qt = w.first_qt + step % w.per_head;
+        if (++qt == w.first_qt + w.per_head) {
+          qt = w.first_qt;
+          ++h;
+        }
         const int pmin = a.q_pos0 + qt * 128;
         const int st = n % ST;
         if (a.table != nullptr && h != lut_h) {
@@ -1685,16 +1739,11 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
         }
         // the statistics come with Q and dO; the scores do after them
         NMB_BAND_WAIT(&q_full[st], (n / ST) & 1, 112);
-        NMB_BAND_WAIT(s_full, n & 1, 113);
+        NMB_BAND_WAIT(&s_full[g], n & 1, 113);
         tc_fence_after();
         uint32_t s[32];
         tmem_ld_32x32(t_row + quarter * 32, s);
         tmem_ld_wait();
-        if (kOwn) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_read);
-        }
         const float* stat = reinterpret_cast<const float*>(smem + L::kStat) + st * kStatBlock + quarter * 32;
         const bool added = a.table != nullptr && (pmin - (w.kv0 + 127) < p.t_last || fabsf(far_bias) > 1e30f);
         const bool whole = w.kv0 + 127 <= pmin && w.kv0 + 127 < a.Skv && (pmin + 127 - w.kv0 < a.window || w.kv0 + 127 < a.sinks);
@@ -1717,43 +1766,47 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
               if (!((see >> k) & 1u)) s[k] = 0;
           }
         }
-        if (kOwn) NMB_BAND_WAIT(dp_full, n & 1, 114);  // P^T and dS^T of the step before have been read
         {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) pk[k] = pack_bf16x2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-          tmem_st_32x16(t_row + kP + quarter * kQuarter, pk);
+          tmem_st_32x16(t_row + quarter * 32, pk);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
-        if (!kOwn) NMB_BAND_WAIT(dp_full, n & 1, 115);
+        if (lane == 0) mbar_arrive(&p_full[g]);
+        NMB_BAND_WAIT(&dp_full[g], n & 1, 115);
         tc_fence_after();
         uint32_t dp[32];
         tmem_ld_32x32(t_row + kDp + quarter * 32, dp);
         tmem_ld_wait();
         uint32_t pk[16];
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 dd = *reinterpret_cast<const float4*>(stat + 128 + k);
-          pk[k / 2] = pack_bf16x2(__uint_as_float(s[k]) * (__uint_as_float(dp[k]) - dd.x),
-                                  __uint_as_float(s[k + 1]) * (__uint_as_float(dp[k + 1]) - dd.y));
-          pk[k / 2 + 1] = pack_bf16x2(__uint_as_float(s[k + 2]) * (__uint_as_float(dp[k + 2]) - dd.z),
-                                      __uint_as_float(s[k + 3]) * (__uint_as_float(dp[k + 3]) - dd.w));
+        for (int k = 0; k < 16; k += 2) {
+          const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(stat + 128 + 2 * k);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int e = 2 * (k + i);
+            float d0, d1;
+            unpack2(mul2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                         fma2(i ? dd.y : dd.x, pack2(-1.f, -1.f), pack2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])))), d0, d1);
+            pk[k + i] = pack_bf16x2(d0, d1);
+          }
         }
-        tmem_st_32x16(t_row + kDs + quarter * kQuarter, pk);
+        tmem_st_32x16(t_row + kDp + quarter * 32, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(ds_full);
+          mbar_arrive(&ds_full[g]);
           mbar_arrive(&q_empty[st]);
         }
       }
       const bool any = w.from < w.to;
       if (any) {
-        NMB_BAND_WAIT(acc_full, n_item & 1, 117);
+        NMB_BAND_WAIT(&acc_full[0], n_item & 1, 117);
+        if (G::kGroups == 2) NMB_BAND_WAIT(&acc_full[1], n_item & 1, 117);
         ++n_item;
         tc_fence_after();
       }
@@ -1767,8 +1820,17 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
           for (int c = 0; c < L::kCols / 16; ++c) {
             uint32_t v[16];
             if (any) {
-              tmem_ld_32x16(t_row + (which == 0 ? kDv : kDk) + quarter * L::kCols + c * 16, v);
-              tmem_ld_wait();
+              const uint32_t at = t_row + (which == 0 ? kDv : kDk) + quarter * L::kCols + c * 16;
+              tmem_ld_32x16(at, v);
+              if (G::kGroups == 2) {
+                uint32_t v2[16];
+                tmem_ld_32x16(at + 128, v2);
+                tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __uint_as_float(v2[k]));
+              } else {
+                tmem_ld_wait();
+              }
             } else {
 #pragma unroll
               for (int k = 0; k < 16; ++k) v[k] = 0;
@@ -1912,6 +1974,13 @@ static BandScratch plan_bwd(BandBwdParams& p, const BandArgs& a) {
   p.n_kt = (a.Skv + 127) / 128;
   p.t_last = a.buckets < 2 ? 0 : a.limit[a.buckets - 2];
   plan_pieces(p);
+  p.by_hqb = FastDiv(a.Hq * a.B);
+  p.by_hq = FastDiv(a.Hq);
+  p.by_group = FastDiv(a.Hq / a.Hkv);
+  p.by_hkvb = FastDiv(a.Hkv * a.B);
+  p.by_hkv = FastDiv(a.Hkv);
+  p.by_sink_pieces = FastDiv(p.sink_pieces);
+  p.by_pieces = FastDiv(p.pieces);
   const long long n_hb = static_cast<long long>(a.Hkv) * a.B;
   const long long slots = (p.sink_pieces > 1 ? p.sink_tiles * p.sink_pieces * n_hb : 0) +
                           (p.pieces > 1 ? (p.n_kt - p.sink_tiles) * p.pieces * n_hb : 0);
@@ -2015,6 +2084,10 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   const long long items = p.pair == 0 ? tiles : p.pair == 2 ? tiles / 2 : static_cast<long long>((p.n_qt + 1) / 2) * a->Hq * a->B;
   if (items > (1 << 30)) return kTooLarge;
   p.n_items = static_cast<int>(items);
+  const int heads = p.pair == 2 ? a->Hq / 2 : a->Hq;
+  p.by_hb = FastDiv(heads * a->B);
+  p.by_heads = FastDiv(heads);
+  p.by_group = FastDiv(a->Hq / a->Hkv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = a->d == 64 ? launch_band_fwd<64>(p, s) : a->d == 96 ? launch_band_fwd<96>(p, s) : launch_band_fwd<128>(p, s);
   if (e == cudaSuccess) ++g_band_launches;
