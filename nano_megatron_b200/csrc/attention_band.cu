@@ -305,6 +305,25 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Results of D = 64 leave through a swizzled tile in shared memory and one tile store: 32 bytes a lane, a line each, took an item
+// 2600 clocks.  (Wider heads leave no room for the tile.)  Rows behind the last are cut off by the tensor map.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* smem_src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// 16 values of row r from column c (a multiple of 16) on
+__device__ __forceinline__ void stage_bf16_16(uint8_t* tile, int r, int c, const uint32_t (&v)[16], float mul) {
+  uint32_t w[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(__uint_as_float(v[2 * k]) * mul, __uint_as_float(v[2 * k + 1]) * mul);
+  *reinterpret_cast<uint4*>(tile + swz128_offset(r, c / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(tile + swz128_offset(r, c / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+}
 // Bounded wait: as mbar_wait, but asleep for up to kNapNs at a time after the first look.  (The first look takes about 50
 // clocks, try_wait 80.)
 constexpr uint32_t kNapNs = 10000;
@@ -412,7 +431,7 @@ constexpr int kComputeWarps = 16, kLoadWarp = 16, kMmaWarp = 17;  // kMmaWarp ow
 #define NMB_BAND_MORE_REGISTERS asm volatile("setmaxnreg.inc.sync.aligned.u32 104;")
 
 struct BandFwdParams {
-  CUtensorMap q_map, k_map, v_map;
+  CUtensorMap q_map, k_map, v_map, o_map, rest_map;
   BandArgs a;
   int pair;     // 0: one tile an item, 1: two neighbouring tiles, 2: two heads
   int n_qt;     // query tiles of a head
@@ -426,10 +445,12 @@ template <int D>
 struct BandFwdSmem {
   static constexpr int kSlabs = (D + 63) / 64;
   static constexpr int kTile = kSlabs * 16384;
-  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr int kStages = D == 64 ? 6 : 4;
   static constexpr int kQ = 0;
   static constexpr int kRing = 2 * kTile;
-  static constexpr int kBar = kRing + kStages * kTile;
+  static constexpr bool kStage = D == 64;  // results through shared memory: O and what was cut off of it, per slot
+  static constexpr int kOut = kRing + kStages * kTile;
+  static constexpr int kBar = kOut + (kStage ? 4 * kTile : 0);
   static constexpr int kNumBars = 2 * kStages + 16;
   static constexpr int kXch = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [2][2 slots][2 halves][128]
   static constexpr int kLut = kXch + 4096;                                     // float [2][entries], then the map
@@ -860,6 +881,12 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* out = band_row(a.o, a.o_st, w.b, row, h) + half * (D / 2);
+      uint8_t* tile = smem + L::kOut + 2 * t * L::kTile;
+      const bool some_rest = q0 < a.rest_rows;
+      if (L::kStage) {
+        if (quad == 0 && half == 0 && lane == 0) store_wait_read();  // the item before has left the tile
+        named_sync(9 + t, 256);
+      }
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[16];
@@ -870,18 +897,33 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = 0;
         }
-        if (row < a.Sq) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+        if (L::kStage) {
+          stage_bf16_16(tile, r, half * (D / 2) + c * 16, o, 1.f);
+        } else if (row < a.Sq) {
           store_bf16_16(out + c * 16, o, 1.f);
-          if (row < a.rest_rows) {
+        }
+        if (some_rest) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float x = __uint_as_float(o[k]);
-              o[k] = __float_as_uint(x - __bfloat162float(__float2bfloat16(x)));
-            }
+          for (int k = 0; k < 16; ++k) {
+            const float x = __uint_as_float(o[k]);
+            o[k] = __float_as_uint(x - __bfloat162float(__float2bfloat16(x)));
+          }
+          if (L::kStage) {
+            stage_bf16_16(tile + L::kTile, r, half * (D / 2) + c * 16, o, 1.f);
+          } else if (row < a.rest_rows) {
             store_bf16_16(rest_row(a, w.b, row, h, D) + half * (D / 2) + c * 16, o, 1.f);
           }
+        }
+      }
+      if (L::kStage) {
+        fence_proxy_async_smem();
+        named_sync(9 + t, 256);
+        if (quad == 0 && half == 0 && lane == 0) {
+          tma_store_4d(&p.o_map, tile, 0, q0, h, w.b);
+          if (some_rest) tma_store_4d(&p.rest_map, tile + L::kTile, 0, q0, h, w.b);
+          store_commit();
         }
       }
       if (n > 0) {
@@ -895,6 +937,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         a.l[stat] = l > 0.f ? log2f(l) : 0.f;
       }
     }
+    if (L::kStage) store_wait();
   }
 
   if (*abort_flag != 0) {  // let the loads in flight land
@@ -958,7 +1001,7 @@ __device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, const fl
 }
 
 struct BandBwdParams {
-  CUtensorMap q_map, k_map, v_map, do_map;
+  CUtensorMap q_map, k_map, v_map, do_map, dq_map, dk_map, dv_map;
   BandArgs a;
   float* stat;      // [B, Hq, n_qt, kStatBlock]
   float* part;      // fp32 dV, dK tiles of key tiles whose rows are split
@@ -1057,11 +1100,13 @@ struct BandDqSmem {
   static constexpr int kQStages = D == 64 ? 2 : 1;
   // K stays until dQ += dS K, V only until dP: where four tiles is all there is room for, three are for K (a ring of two
   // pairs left the loads of K exposed: 1640 of 4020 clocks a tile were spent waiting at d = 128)
-  static constexpr int kStagesK = D == 64 ? 4 : 3, kStagesV = D == 64 ? 4 : 1;
+  static constexpr int kStagesK = 3, kStagesV = D == 64 ? 3 : 1;
   static constexpr int kStages = kStagesK + kStagesV;
   static constexpr int kQ = 0;                     // Q, dO per stage
   static constexpr int kRing = 2 * kQStages * kTile;  // the stages of K, then those of V
-  static constexpr int kStat = kRing + kStages * kTile;  // per stage of Q
+  static constexpr bool kStage = D == 64;  // dQ through shared memory
+  static constexpr int kOut = kRing + kStages * kTile;
+  static constexpr int kStat = kOut + (kStage ? kTile : 0);  // per stage of Q
   static constexpr int kBar = kStat + kQStages * kStatBlock * 4;
   static constexpr int kNumBars = 2 * kStages + 2 * kQStages + 11;
   static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;  // float [entries], the map
@@ -1403,6 +1448,10 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         ++n_item;
         tc_fence_after();
       }
+      if (L::kStage) {
+        if (threadIdx.x == 0) store_wait_read();  // the item before has left the tile
+        together();
+      }
       if (has_cols) {
         __nv_bfloat16* out = band_row(a.dq, a.dq_st, w.b, row, w.h) + quarter * L::kCols;
 #pragma unroll
@@ -1423,7 +1472,19 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
 #pragma unroll
             for (int k = 0; k < 16; ++k) v[k] = 0;
           }
-          if (valid) store_bf16_16(out + c * 16, v, a.scale);
+          if (L::kStage) {
+            stage_bf16_16(smem + L::kOut, r, quarter * L::kCols + c * 16, v, a.scale);
+          } else if (valid) {
+            store_bf16_16(out + c * 16, v, a.scale);
+          }
+        }
+      }
+      if (L::kStage) {
+        fence_proxy_async_smem();
+        together();
+        if (threadIdx.x == 0) {
+          tma_store_4d(&p.dq_map, smem + L::kOut, 0, w.q0, w.h, w.b);
+          store_commit();
         }
       }
       if (n > 0) {
@@ -1447,6 +1508,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         together();
       }
     }
+    if (L::kStage) store_wait();
   }
 
   if (*abort_flag != 0) {
@@ -1473,7 +1535,9 @@ struct BandDkvSmem {
   static constexpr int kKvStages = D == 64 ? 2 : 1;  // K, V
   static constexpr int kK = 0;
   static constexpr int kRing = 2 * kKvStages * kTile;
-  static constexpr int kStat = kRing + 2 * kStages * kTile;
+  static constexpr bool kStage = D == 64;  // dV, dK through shared memory
+  static constexpr int kOut = kRing + 2 * kStages * kTile;
+  static constexpr int kStat = kOut + (kStage ? 2 * kTile : 0);
   static constexpr int kBar = kStat + kStages * kStatBlock * 4;
   static constexpr int kNumBars = 2 * kStages + 2 * kKvStages + 11;
   static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;
@@ -1810,6 +1874,11 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
         ++n_item;
         tc_fence_after();
       }
+      const bool staged = L::kStage && w.slot < 0;
+      if (staged) {
+        if (threadIdx.x == 0) store_wait_read();  // the item before has left the tiles
+        together();
+      }
       if (has_cols) {
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -1838,10 +1907,21 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
             if (w.slot >= 0) {
               st_global_32(part + c * 16, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
               st_global_32(part + c * 16 + 8, v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]);
+            } else if (L::kStage) {
+              stage_bf16_16(smem + L::kOut + which * L::kTile, r, quarter * L::kCols + c * 16, v, mul);
             } else if (j < a.Skv) {
               store_bf16_16(out + c * 16, v, mul);
             }
           }
+        }
+      }
+      if (staged) {
+        fence_proxy_async_smem();
+        together();
+        if (threadIdx.x == 0) {
+          tma_store_4d(&p.dv_map, smem + L::kOut, 0, w.kv0, w.hk, w.b);
+          tma_store_4d(&p.dk_map, smem + L::kOut + L::kTile, 0, w.kv0, w.hk, w.b);
+          store_commit();
         }
       }
       if (any) {
@@ -1850,6 +1930,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
         if (lane == 0) mbar_arrive(acc_empty);
       }
     }
+    if (L::kStage) store_wait();
   }
 
   if (*abort_flag != 0) {
@@ -2075,6 +2156,11 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   if (make_band_map(&p.q_map, a->q, a->q_st, a->d, a->Sq, a->Hq, a->B)) return 101;
   if (make_band_map(&p.k_map, a->k, a->k_st, a->d, a->Skv, a->Hkv, a->B)) return 102;
   if (make_band_map(&p.v_map, a->v, a->v_st, a->d, a->Skv, a->Hkv, a->B)) return 103;
+  if (make_band_map(&p.o_map, a->o, a->o_st, a->d, a->Sq, a->Hq, a->B)) return 105;
+  if (a->rest_rows > 0) {
+    const long long row = static_cast<long long>(a->Hq) * a->d;
+    if (make_band_map(&p.rest_map, a->o_rest, BandStride{a->rest_rows * row, row, a->d}, a->d, a->rest_rows, a->Hq, a->B)) return 106;
+  }
   p.n_qt = (a->Sq + 127) / 128;
   p.s_pad = p.n_qt * 128;
   p.t_last = a->table == nullptr ? 0 : a->limit[a->buckets - 2];
@@ -2106,6 +2192,9 @@ extern "C" int nmb_band_bwd(const BandArgs* a, void* stream) {
   if (make_band_map(&p.k_map, a->k, a->k_st, a->d, a->Skv, a->Hkv, a->B)) return 102;
   if (make_band_map(&p.v_map, a->v, a->v_st, a->d, a->Skv, a->Hkv, a->B)) return 103;
   if (make_band_map(&p.do_map, a->dout, a->dout_st, a->d, a->Sq, a->Hq, a->B)) return 104;
+  if (make_band_map(&p.dq_map, a->dq, a->dq_st, a->d, a->Sq, a->Hq, a->B)) return 107;
+  if (make_band_map(&p.dk_map, a->dk, a->dk_st, a->d, a->Skv, a->Hkv, a->B)) return 108;
+  if (make_band_map(&p.dv_map, a->dv, a->dv_st, a->d, a->Skv, a->Hkv, a->B)) return 109;
   const long long n_hb = static_cast<long long>(a->Hkv) * a->B;
   const long long dq_items = static_cast<long long>(p.n_qt) * a->Hq * a->B;
   const long long dkv_items = (static_cast<long long>(p.sink_tiles) * p.sink_pieces +
