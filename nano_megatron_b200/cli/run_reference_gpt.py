@@ -35,7 +35,11 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--lr", type=float, default=1e-3)
     p.add_argument("--weight-decay", type=float, default=0.01)
     p.add_argument("--gelu", action="store_true", help="GELU MLP instead of SwiGLU")
-    p.add_argument("--learned-pos", action="store_true", help="learned absolute positions instead of RoPE")
+    positions = p.add_mutually_exclusive_group()
+    positions.add_argument("--learned-pos", action="store_true", help="learned absolute positions instead of RoPE")
+    positions.add_argument("--relative-pos", action="store_true", help="learned relative position bias instead of RoPE")
+    p.add_argument("--window", type=int, default=None, help="attention sees the last WINDOW positions")
+    p.add_argument("--sinks", type=int, default=0, help="... and the first SINKS tokens")
     p.add_argument("--tied", action="store_true", help="tie input and output embeddings")
     p.add_argument("--bias", action="store_true")
     p.add_argument("--fused-qkv", action="store_true")
@@ -49,7 +53,8 @@ def main(argv: list[str] | None = None) -> int:
     cfg = ReferenceGPTConfig(
         vocab_size=args.vocab, max_seq_len=args.seq, hidden_size=args.hidden, num_layers=args.layers,
         num_heads=args.heads, ffn_hidden_size=args.ffn, use_bias=args.bias, tie_word_embeddings=args.tied,
-        position_embedding_type="learned_absolute" if args.learned_pos else "rope",
+        position_embedding_type="learned_absolute" if args.learned_pos else "relative" if args.relative_pos else "rope",
+        attention_window=args.window, attention_sinks=args.sinks,
         gated_linear_unit=not args.gelu, activation_func="gelu" if args.gelu else "swiglu",
         use_fused_qkv=args.fused_qkv, attn_backend="unfused")
     device = torch.device(args.device)

@@ -38,6 +38,9 @@ FIELD_MAP = [
 ]
 
 
+_POSITIONS = {"rope": "RoPE", "learned_absolute": "learned absolute", "relative": "relative bias"}
+
+
 def expected_parameter_count(cfg: ReferenceGPTConfig) -> int:
     """Closed-form parameter count of the decoder described by ``cfg``."""
     h, f, v, layers = cfg.hidden_size, cfg.ffn_hidden_size, cfg.vocab_size, cfg.num_layers
@@ -52,6 +55,8 @@ def expected_parameter_count(cfg: ReferenceGPTConfig) -> int:
     total += v * h                                  # token embedding
     if cfg.position_embedding_type == "learned_absolute":
         total += cfg.max_seq_len * h
+    if cfg.position_embedding_type == "relative":
+        total += layers * cfg.num_heads * cfg.relative_buckets
     if not cfg.tie_word_embeddings:
         total += v * h                              # LM head
     return total
@@ -105,7 +110,7 @@ def verify(cfg: ReferenceGPTConfig, megatron_path: Optional[str] = None, *, forw
     counted, expected = count_parameters(cfg), expected_parameter_count(cfg)
     print(f"\nparameters: {counted:,} (closed form {expected:,})", file=out)
     ok &= counted == expected
-    print(f"position embedding : {'RoPE' if cfg.position_embedding_type == 'rope' else 'learned absolute'}", file=out)
+    print(f"position embedding : {_POSITIONS[cfg.position_embedding_type]}", file=out)
     print(f"MLP activation     : {'SwiGLU' if cfg.gated_linear_unit else 'GELU (erf)'}", file=out)
     print(f"linear bias        : {'on' if cfg.use_bias else 'off'}", file=out)
     print(f"normalization      : {cfg.normalization}", file=out)

@@ -113,10 +113,11 @@ class PipelineTrainer:
         """Every parameter's gradient is accumulated into its bucket buffer by the
         backward kernels themselves (``main_grad``).  Parameters whose gradient
         comes back through autograd (replicated parameters under sequence
-        parallelism, whose hook reduces them over the TP group) need the eager
-        schedule: the graphed backward of a later stage asks autograd only for the
+        parallelism, whose hook reduces them over the TP group; the relative
+        position bias) need the eager schedule: the graphed backward of a later stage asks autograd only for the
         gradient of the stage input."""
         return all(getattr(p, "main_grad", None) is not None and not getattr(p, "_nmb_sp_replicated", False)
+                   and not getattr(p, "_nmb_through_autograd", False)
                    for p in self.stage.parameters() if p.requires_grad)
 
     @property

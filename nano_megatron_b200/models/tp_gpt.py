@@ -21,9 +21,11 @@ from torch.nn import Parameter
 
 from ..ops import functional as OF
 from ..parallel.attention_backend import (
+    flash_banded_attention,
     flash_causal_attention,
     flash_ring_causal_attention,
     resolve_attention_backend,
+    unfused_banded_attention,
     unfused_causal_attention,
 )
 from ..parallel.context import ParallelContext
@@ -97,6 +99,12 @@ class TPCausalSelfAttention(nn.Module):
                                                          sequence_parallel=sp))
         self.out_proj = RowParallelLinear(ref_attn.out_proj.weight, ref_attn.out_proj.bias, rank, tp, group,
                                           backend, sequence_parallel=sp)
+        self.banded = ref_attn.banded
+        self.rel_bias: Optional[Parameter] = None
+        if ref_attn.rel_bias is not None:
+            first = rank * self.local_num_heads
+            self.rel_bias = Parameter(ref_attn.rel_bias.data[first:first + self.local_num_heads].clone())
+            self.rel_bias._nmb_through_autograd = True  # its gradient comes back from the attention's node
         self.rotary_emb = self.config.position_embedding_type == "rope"
         if self.rotary_emb:
             self.freqs = precompute_freqs_cis(self.config.rotary_dim, self.config.max_seq_len,
@@ -135,7 +143,7 @@ class TPCausalSelfAttention(nn.Module):
 
     def forward(self, x: Tensor, positions: Optional[Tensor] = None, *, residual: Optional[Tensor] = None) -> Tensor:
         if self._native_ok(x):
-            return self._forward_native(x, positions, residual)
+            return (self._forward_banded if self.banded else self._forward_native)(x, positions, residual)
         q, k, v = self._project(x)
         q = self._split_heads(q, self.local_num_heads)
         k = self._split_heads(k, self.local_num_kv_heads)
@@ -148,7 +156,17 @@ class TPCausalSelfAttention(nn.Module):
         backend = resolve_attention_backend(requested=getattr(self.config, "attn_backend", "auto"), dtype=q.dtype,
                                             device=q.device, return_activations=False)
         dropout_p = float(getattr(self.config, "attention_dropout", 0.0))
-        if backend == "flash" and self._cp_size > 1:
+        if self.banded:
+            start = 0
+            if self._cp_size > 1:
+                start = self._cp_rank * q.size(2)
+                k, v = (gather_from_context_parallel_region(t, self._cp_group, self._cp_backend, self._cp_rank, self._cp_size,
+                                                            seq_dim=2) for t in (k, v))
+            if backend == "flash":
+                context = flash_banded_attention(q, k, v, scale=self.scale, query_start=start, dropout_p=dropout_p, **self._band())
+            else:
+                context = unfused_banded_attention(q, k, v, scale=self.scale, query_start=start, **self._band())
+        elif backend == "flash" and self._cp_size > 1:
             context = flash_ring_causal_attention(q, k, v, scale=self.scale, cp_group=self._cp_group,
                                                   cp_rank=self._cp_rank, cp_size=self._cp_size,
                                                   backend=self._cp_backend, dropout_p=dropout_p)
@@ -164,6 +182,47 @@ class TPCausalSelfAttention(nn.Module):
         else:
             context = unfused_causal_attention(q, k, v, scale=self.scale)
         return self.out_proj(self._merge_heads(context), residual=residual)
+
+    def _band(self) -> dict:
+        return dict(window=self.config.attention_window, sinks=self.config.attention_sinks, table=self.rel_bias,
+                    max_distance=self.config.relative_max_distance)
+
+    def _rotate(self, q: Tensor, k: Tensor, positions: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+        """Rotary embedding of ``[B, S, heads, d]`` views by kernels of their own."""
+        if not self.rotary_emb or positions is None:
+            return q, k
+        if self._inv_freq_dev is None or self._inv_freq_dev.device != q.device:
+            half = torch.arange(0, self.config.rotary_dim, 2).float() / self.config.rotary_dim
+            self._inv_freq_dev = (1.0 / (float(self.config.rotary_base) ** half)).to(q.device)
+        pos = positions.contiguous()
+        return OF.rope_bshd(q, pos, self._inv_freq_dev), OF.rope_bshd(k, pos, self._inv_freq_dev)
+
+    def _forward_banded(self, x: Tensor, positions: Optional[Tensor], residual: Optional[Tensor]) -> Tensor:
+        """bf16 GPU path of attention inside a window and / or with a relative position bias.  The kernels read the slices of
+        the packed projection in place and write the gradients of all three into one buffer.  Under context parallelism the
+        keys and values of all ranks are gathered; a rank's queries are a shard of the sequence to the kernels."""
+        from ..ops.attention import split_packed_qkv
+        from ..ops.band_attention import relative_bias_attention, window_attention
+
+        d, hq, hkv = self.head_dim, self.local_num_heads, self.local_num_kv_heads
+        if self.config.use_fused_qkv:
+            q, k, v = split_packed_qkv(self.qkv_proj(x), hq, hkv, d)
+        else:
+            q, k, v = (t.unflatten(-1, (-1, d)) for t in (self.q_proj(x), self.k_proj(x), self.v_proj(x)))
+        q, k = self._rotate(q, k, positions)
+        b, s = q.shape[:2]
+        start = 0
+        if self._cp_size > 1:
+            start = self._cp_rank * s
+            k, v = (gather_from_context_parallel_region(t, self._cp_group, self._cp_backend, self._cp_rank, self._cp_size,
+                                                        seq_dim=1) for t in (k, v))
+        window, sinks = self.config.attention_window, self.config.attention_sinks
+        if self.rel_bias is None:
+            context = window_attention(q, k, v, self.scale, window=window, sinks=sinks, query_start=start)
+        else:
+            context = relative_bias_attention(q, k, v, self.rel_bias, self.scale, max_distance=self.config.relative_max_distance,
+                                              window=window, sinks=sinks, query_start=start)
+        return self.out_proj(context.view(b, s, hq * d), residual=residual)
 
     def _rope_spec(self, device: torch.device, positions: Tensor, rope_cols: int):
         """Table of (cos, sin) per position and pair, cached per device, plus the
@@ -224,13 +283,7 @@ class TPCausalSelfAttention(nn.Module):
             q, k, v = self.q_proj(x), self.k_proj(x), self.v_proj(x)
             b, s, _ = q.shape
             q, k, v = q.view(b, s, hq, d), k.view(b, s, hkv, d), v.view(b, s, hkv, d)
-        if self.rotary_emb and positions is not None:
-            if self._inv_freq_dev is None or self._inv_freq_dev.device != x.device:
-                half = torch.arange(0, self.config.rotary_dim, 2).float() / self.config.rotary_dim
-                self._inv_freq_dev = (1.0 / (float(self.config.rotary_base) ** half)).to(x.device)
-            pos = positions.contiguous()
-            q = OF.rope_bshd(q, pos, self._inv_freq_dev)
-            k = OF.rope_bshd(k, pos, self._inv_freq_dev)
+        q, k = self._rotate(q, k, positions)
         if self._cp_size > 1:
             from ..parallel.cp_attention import cp_flash_attention
             context = cp_flash_attention(q, k, v, scale=self.scale, cp_group=self._cp_group, cp_rank=self._cp_rank,

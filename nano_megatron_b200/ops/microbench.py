@@ -103,6 +103,28 @@ def bench_attn(args) -> None:
         _bench_library_attention(args, qkv, g, fwd_flops)
 
 
+def bench_band(args) -> None:
+    """Banded attention of ``--batch`` x ``--seq`` tokens, ``--heads`` heads of ``--dim``: a window, a relative bias, both."""
+    from .band_attention import relative_bias_attention, window_attention
+
+    b, s, h, d = args.batch, args.seq, args.heads, args.dim
+    q, k, v = (torch.randn(b, s, h, d, device="cuda").to(torch.bfloat16).requires_grad_(True) for _ in range(3))
+    table = torch.randn(h, 32, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    g = torch.randn_like(q)
+    scale, window, sinks = 1.0 / math.sqrt(d), args.window, args.sinks
+    in_window = sum(min(p + 1, window + min(sinks, max(0, p + 1 - window))) for p in range(s))
+    calls = {f"window {window}, {sinks} sinks": (lambda: window_attention(q, k, v, scale, window=window, sinks=sinks), (q, k, v), in_window),
+             "relative bias": (lambda: relative_bias_attention(q, k, v, table, scale), (q, k, v, table), s * (s + 1) // 2),
+             "relative bias in the window": (lambda: relative_bias_attention(q, k, v, table, scale, window=window, sinks=sinks),
+                                             (q, k, v, table), in_window)}
+    for name, (call, leaves, pairs) in calls.items():
+        flops = 4.0 * b * h * pairs * d
+        with torch.no_grad():
+            _report(f"{name} fwd b{b} s{s} h{h} d{d}", _timed(call, args.iters), flops)
+        out = call()
+        _report(f"{name} bwd", _timed(lambda: torch.autograd.grad(out, leaves, g, retain_graph=True), args.iters), 2.5 * flops)
+
+
 def _bench_library_attention(args, qkv, g, fwd_flops) -> None:
     """The same workload through the flash-attn package, as a yardstick only (it is not
     on any path of this framework)."""
@@ -164,7 +186,7 @@ def bench_adamw(args) -> None:
 
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("kernel", choices=["gemm", "attn", "norm", "ce", "adamw", "all"])
+    ap.add_argument("kernel", choices=["gemm", "attn", "band", "norm", "ce", "adamw", "all"])
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--m", type=int, default=4096)
     ap.add_argument("--n", type=int, default=4096)
@@ -176,6 +198,8 @@ def main(argv=None) -> int:
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--heads", type=int, default=16)
     ap.add_argument("--dim", type=int, default=64)
+    ap.add_argument("--window", type=int, default=512)
+    ap.add_argument("--sinks", type=int, default=4)
     ap.add_argument("--rows", type=int, default=4096)
     ap.add_argument("--hidden", type=int, default=1024)
     ap.add_argument("--vocab", type=int, default=50304)
@@ -184,7 +208,7 @@ def main(argv=None) -> int:
     if not torch.cuda.is_available():
         print("no CUDA device")
         return 1
-    todo = ["gemm", "attn", "norm", "ce", "adamw"] if args.kernel == "all" else [args.kernel]
+    todo = ["gemm", "attn", "band", "norm", "ce", "adamw"] if args.kernel == "all" else [args.kernel]
     for name in todo:
         globals()[f"bench_{name}"](args)
     torch.cuda.synchronize()

@@ -1,4 +1,4 @@
-"""Attention backend resolution and the three attention entry points.
+"""Attention backend resolution and the attention entry points.
 
 Names and tensor conventions (``[B, heads, S, d]`` in and out) follow the
 reference (nano_megatron/parallel/attention_backend.py:22-635).  ``"flash"``
@@ -104,6 +104,41 @@ def flash_causal_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, dro
     _check_qkv(q, k, v)
     _require_flash(q, dropout_p)
     out = flash_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), scale)
+    return out.transpose(1, 2)
+
+
+def unfused_banded_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, window: Optional[int] = None, sinks: int = 0,
+                             table: Optional[Tensor] = None, max_distance: int = 128, query_start: int = 0) -> Tensor:
+    """Causal attention inside a window (with sinks) and / or with a relative position bias, as scores -> softmax -> @V; the
+    queries are rows from position ``query_start`` on.  ``[B, heads, S, d]``, equal numbers of heads."""
+    from ..reference.layers import banded_attn_scores, softmax_last
+
+    _check_qkv(q, k, v)
+    if q.shape[1] != k.shape[1]:
+        raise ValueError(f"q/k heads must match; got q={tuple(q.shape)}, k={tuple(k.shape)}")
+    if query_start < 0 or query_start + q.size(2) > k.size(2):
+        raise ValueError(f"query_start ({query_start}) + S_q ({q.size(2)}) exceeds S_k ({k.size(2)})")
+    scores = banded_attn_scores(q, k, scale, window=window, sinks=sinks, table=table, max_distance=max_distance,
+                                query_start=query_start)
+    return torch.matmul(softmax_last(scores), v)
+
+
+def flash_banded_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, window: Optional[int] = None, sinks: int = 0,
+                           table: Optional[Tensor] = None, max_distance: int = 128, query_start: int = 0,
+                           dropout_p: float = 0.0) -> Tensor:
+    """The same on the kernels of ``csrc/attention_band.cu``; ``k`` / ``v`` may have fewer (grouped) heads."""
+    from ..ops.band_attention import relative_bias_attention, window_attention
+
+    _check_qkv(q, k, v)
+    _require_flash(q, dropout_p)
+    if window is None and table is None:
+        raise ValueError("neither a window nor a bias table: use flash_causal_attention")
+    q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+    if table is None:
+        out = window_attention(q, k, v, scale, window=window, sinks=sinks, query_start=query_start)
+    else:
+        out = relative_bias_attention(q, k, v, table, scale, max_distance=max_distance, window=window, sinks=sinks,
+                                      query_start=query_start)
     return out.transpose(1, 2)
 
 

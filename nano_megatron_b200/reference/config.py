@@ -25,7 +25,7 @@ class ReferenceGPTConfig:
     tie_word_embeddings: bool = False
     dtype: torch.dtype = torch.float32
 
-    position_embedding_type: Literal["learned_absolute", "rope"] = "rope"
+    position_embedding_type: Literal["learned_absolute", "rope", "relative"] = "rope"
     rotary_dim: Optional[int] = None
     rotary_base: int = 10000
     activation_func: Literal["gelu", "swiglu"] = "swiglu"  # informational; see gated_linear_unit
@@ -37,6 +37,13 @@ class ReferenceGPTConfig:
     hidden_dropout: float = 0.0
     attention_dropout: float = 0.0
     attn_backend: Literal["auto", "flash", "unfused"] = "auto"
+
+    # Banded attention (no counterpart in the reference project): a query sees the last ``attention_window`` positions and the
+    # first ``attention_sinks`` tokens; "relative" positions are a learned bias per head and bucket of distances in every layer.
+    attention_window: Optional[int] = None
+    attention_sinks: int = 0
+    relative_buckets: int = 32
+    relative_max_distance: int = 128
 
     def __post_init__(self) -> None:
         if self.hidden_size % self.num_heads != 0:
@@ -51,6 +58,14 @@ class ReferenceGPTConfig:
             self.rotary_dim = head_dim
         if self.num_query_groups is None:
             self.num_query_groups = self.num_heads
+        if self.attention_window is not None and self.attention_window < 1:
+            raise ValueError(f"attention_window must be at least 1, got {self.attention_window}")
+        if self.attention_sinks < 0 or (self.attention_sinks > 0 and self.attention_window is None):
+            raise ValueError(f"attention_sinks ({self.attention_sinks}) must not be negative and need an attention_window")
+        if self.position_embedding_type == "relative" and not \
+                2 <= self.relative_buckets < 2 * self.relative_max_distance + 2:
+            raise ValueError(f"relative_max_distance ({self.relative_max_distance}) must be above half of relative_buckets "
+                             f"({self.relative_buckets}), of which there must be two at least")
         # Modules are always built in fp32; callers cast afterwards (as the
         # reference's benchmarks do with ``model.to(torch.bfloat16)``).
         self.dtype = torch.float32

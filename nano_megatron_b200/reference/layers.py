@@ -63,6 +63,23 @@ def causal_attn_scores(q: Tensor, k: Tensor, scale: float) -> Tensor:
     return scores.masked_fill(future, torch.finfo(scores.dtype).min)
 
 
+def banded_attn_scores(q: Tensor, k: Tensor, scale: float, *, window: Optional[int] = None, sinks: int = 0,
+                       table: Optional[Tensor] = None, max_distance: int = 128, query_start: int = 0) -> Tensor:
+    """Causal scores of ``q`` rows that start at position ``query_start``: inside a window (keys of the last ``window``
+    positions and the first ``sinks`` ones) and with a bias ``table[head, bucket(distance)]`` where these are given."""
+    from ..ops.band_attention import relative_position_buckets
+
+    scores = torch.matmul(q, k.transpose(-2, -1)) * scale
+    key = torch.arange(k.size(-2), device=q.device)
+    distance = torch.arange(query_start, query_start + q.size(-2), device=q.device)[:, None] - key
+    if table is not None:
+        scores = scores + table.to(scores.dtype)[:, relative_position_buckets(distance.clamp(min=0), table.shape[1], max_distance)]
+    hidden = distance < 0
+    if window is not None:
+        hidden = hidden | ((distance >= window) & (key >= sinks))
+    return scores.masked_fill(hidden, torch.finfo(scores.dtype).min)
+
+
 def softmax_last(x: Tensor) -> Tensor:
     return torch.softmax(x, dim=-1)
 
@@ -90,6 +107,10 @@ class CausalSelfAttention(nn.Module):
             self.k_proj = nn.Linear(config.hidden_size, kv_dim, bias=qkv_bias)
             self.v_proj = nn.Linear(config.hidden_size, kv_dim, bias=qkv_bias)
         self.out_proj = nn.Linear(config.hidden_size, config.hidden_size, bias=config.use_bias)
+        self.banded = config.attention_window is not None or config.position_embedding_type == "relative"
+        self.rel_bias: Optional[nn.Parameter] = None
+        if config.position_embedding_type == "relative":
+            self.rel_bias = nn.Parameter(torch.zeros(config.num_heads, config.relative_buckets))
         self.rotary_emb = config.position_embedding_type == "rope"
         if self.rotary_emb:
             self.freqs = precompute_freqs_cis(config.rotary_dim, config.max_seq_len, theta=config.rotary_base)
@@ -111,6 +132,7 @@ class CausalSelfAttention(nn.Module):
 
     def forward(self, x: Tensor, positions: Optional[Tensor] = None, return_activations: bool = False):
         from ..parallel.attention_backend import (
+            flash_banded_attention,
             flash_causal_attention,
             resolve_attention_backend,
             unfused_causal_attention,
@@ -136,7 +158,16 @@ class CausalSelfAttention(nn.Module):
             return_activations=return_activations,
         )
         scores = probs = None
-        if backend == "flash":
+        if self.banded:
+            band = dict(window=self.config.attention_window, sinks=self.config.attention_sinks, table=self.rel_bias,
+                        max_distance=self.config.relative_max_distance)
+            if backend == "flash":
+                context = flash_banded_attention(q, k, v, scale=self.scale, dropout_p=self.config.attention_dropout, **band)
+            else:
+                scores = banded_attn_scores(q, k, self.scale, **band)
+                probs = softmax_last(scores)
+                context = torch.matmul(probs, v)
+        elif backend == "flash":
             context = flash_causal_attention(q, k, v, scale=self.scale, dropout_p=self.config.attention_dropout)
         elif return_activations:
             scores = causal_attn_scores(q, k, scale=self.scale)

@@ -25,7 +25,7 @@ from torch import Tensor, nn
 
 from ..reference.config import ReferenceGPTConfig
 
-_COLUMN = ("q_proj", "k_proj", "v_proj", "lm_head", "tok_emb")
+_COLUMN = ("q_proj", "k_proj", "v_proj", "lm_head", "tok_emb", "rel_bias")
 
 
 def _kind(name: str, cfg: ReferenceGPTConfig) -> str:
