@@ -392,6 +392,22 @@ __device__ __forceinline__ bool band_wait_all(volatile int* abort_flag, int* sta
   if (try_wait_all(bars...)) return true;
   return (band_wait(bars.bar, bars.parity, abort_flag, status, where) && ...);
 }
+// Which comes first: all of `bars` (0) or `other` (1); 2 on failure
+template <class... Bars>
+__device__ __forceinline__ int band_wait_first(volatile int* abort_flag, int* status, int where, BandBar other, const Bars&... bars) {
+  if ((mbar_test_wait(bars.bar, bars.parity) && ...)) return 0;
+  const long long t0 = clock64();
+  while (true) {
+    if (mbar_test_wait(other.bar, other.parity)) return 1;
+    if ((mbar_test_wait(bars.bar, bars.parity) && ...)) return 0;
+    if (*abort_flag != 0) return 2;
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      report_status(status, kMbarTimeout, where);
+      *abort_flag = 1;
+      return 2;
+    }
+  }
+}
 // The compute warps' waits.  After one has failed the others are passed by and the loops run to their end on whatever is
 // there: every warp comes to every named barrier, whichever of them gave up, and no warp waits at one for another that left.
 #define NMB_BAND_WAIT(bar, parity, where)                                            \
@@ -1011,6 +1027,7 @@ struct BandBwdParams {
   int t_last;
   int sink_tiles;   // dK, dV: key tiles that hold sinks, their pieces, the pieces of the others
   int sink_pieces, pieces;
+  int first_seen;   // the first of the others that a row sees
   FastDiv by_hqb, by_hq, by_group;                        // dQ: query heads times batches, query heads; query heads of a key head
   FastDiv by_hkvb, by_hkv, by_sink_pieces, by_pieces;     // dK, dV: the same of key heads, and the pieces
 };
@@ -1019,15 +1036,16 @@ struct BandBwdParams {
 // A block per query tile; D / 8 lanes a row (16 bytes each of dO, O and what was cut off of it), a thread's rows in flight together.
 // In the dQ kernel, a thread per quarter row, the same loads hit a line per lane and cost an item 4000 clocks.
 template <int D>
-__global__ void __launch_bounds__(256) band_stat_kernel(const __grid_constant__ BandBwdParams p) {
+__global__ void __launch_bounds__(256, 2) band_stat_kernel(const __grid_constant__ BandBwdParams p) {
   pdl_enter();
   const BandArgs& a = p.a;
   constexpr int kLanes = D == 64 ? 8 : 16;  // 12 of 16 at D = 96
   constexpr int kRowsAtOnce = 256 / kLanes, kStatRows = 128 / kRowsAtOnce;
   const int sub = threadIdx.x / kLanes, part = threadIdx.x % kLanes;
-  const long long tile = blockIdx.x;  // (b * Hq + h) * n_qt + qt
-  const int qt = static_cast<int>(tile % p.n_qt), h = static_cast<int>(tile / p.n_qt % a.Hq);
-  const int b = static_cast<int>(tile / p.n_qt / a.Hq);
+  // heads run fastest: their rows lie next to one another in memory
+  int rest_of, h;
+  const int qt = p.by_hqb.quot(static_cast<int>(blockIdx.x), rest_of), b = p.by_hq.quot(rest_of, h);
+  const long long tile = (static_cast<long long>(b) * a.Hq + h) * p.n_qt + qt;
   const bool mine = part * 8 < D;
   uint4 o[kStatRows], rest[kStatRows], g[kStatRows];
 #pragma unroll
@@ -1368,7 +1386,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         const bool added = near || (a.table != nullptr && fabsf(far_bias) > 1e30f);
         const bool whole = kv0 + 127 <= pmin && kv0 + 127 < a.Skv && (pmin + 127 - kv0 < a.window || kv0 + 127 < a.sinks);
         // weights, in place of the scores
-        if (whole && !added && w.q0 + 128 <= a.Sq) {  // every row sees finite scores: no weight has to come out as 0
+        if (!added && w.q0 + 128 <= a.Sq) {  // every row sees finite scores: no weight has to come out as 0
           exps32<true>(s, pack2(sl2, sl2), pack2(c_far, c_far));
         } else if (!added) {
           exps32<false>(s, pack2(sl2, sl2), pack2(c_far, c_far));
@@ -1539,7 +1557,7 @@ struct BandDkvSmem {
   static constexpr int kOut = kRing + 2 * kStages * kTile;
   static constexpr int kStat = kOut + (kStage ? 2 * kTile : 0);
   static constexpr int kBar = kStat + kStages * kStatBlock * 4;
-  static constexpr int kNumBars = 2 * kStages + 2 * kKvStages + 11;
+  static constexpr int kNumBars = 4 * kStages + 2 * kKvStages + 11;
   static constexpr int kLut = kBar + ((kNumBars * 8 + 16 + 127) / 128) * 128;
   static constexpr int kCols = D == 96 ? 32 : D / 4;  // as in the dQ kernel
 };
@@ -1550,6 +1568,12 @@ struct DkvItem {
   int first_qt, per_head;
   int from, to;    // steps of this piece: step / per_head = head of the group, step % per_head = query tile
 };
+// The n-th of the key tiles without sinks.  The first that a row sees comes first: it has the most rows; tiles before it (which
+// a shard's window has left behind) have none and come last.
+__host__ __device__ __forceinline__ int other_tile(const BandBwdParams& p, int n) {
+  const int seen = p.first_seen + n;
+  return seen < p.n_kt ? seen : seen - p.n_kt + p.sink_tiles;
+}
 __device__ __forceinline__ DkvItem dkv_item(const BandBwdParams& p, int item) {
   const BandArgs& a = p.a;
   DkvItem w;
@@ -1558,7 +1582,8 @@ __device__ __forceinline__ DkvItem dkv_item(const BandBwdParams& p, int item) {
   const int rank = sink ? item : item - sink_items, pieces = sink ? p.sink_pieces : p.pieces;
   int hb, piece;
   const int at = p.by_hkvb.quot(rank, hb);
-  const int tile = (sink ? 0 : p.sink_tiles) + (sink ? p.by_sink_pieces : p.by_pieces).quot(at, piece);
+  const int nth = (sink ? p.by_sink_pieces : p.by_pieces).quot(at, piece);
+  const int tile = sink ? nth : other_tile(p, nth);
   w.slot = pieces == 1 ? -1 : sink ? rank : (p.sink_pieces > 1 ? sink_items : 0) + rank;
   w.b = p.by_hkv.quot(hb, w.hk);
   w.kv0 = tile * 128;
@@ -1606,7 +1631,9 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* q_full = bars;              // [ST]
   uint64_t* q_empty = bars + ST;        // [ST] the issuers + the warps that read the statistics
-  uint64_t* kv_full = bars + 2 * ST;    // [KS]
+  uint64_t* do_full = bars + 2 * ST;    // [ST]
+  uint64_t* do_empty = bars + 3 * ST;   // [ST] the issuers
+  uint64_t* kv_full = bars + 4 * ST;    // [KS]
   uint64_t* kv_empty = kv_full + KS;    // [KS] the issuers
   uint64_t* s_full = kv_empty + KS;     // [groups], as all that follow
   uint64_t* dp_full = s_full + 2;
@@ -1630,6 +1657,8 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
     for (int s = 0; s < ST; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], G::kGroups + kComputeWarps);
+      mbar_init(&do_full[s], 1);
+      mbar_init(&do_empty[s], G::kGroups);
     }
     for (int s = 0; s < KS; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -1690,22 +1719,27 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
           }
         }
         const int st = n % ST, use = n / ST;
-        if (use > 0 && !band_wait(&q_empty[st], (use - 1) & 1, abort_flag, a.status, 102)) break;
         const int h = x.w.hk * group + x.step / x.w.per_head, qt = x.w.first_qt + x.step % x.w.per_head;
-        mbar_expect_tx(&q_full[st], 2 * L::kTile + stat_bytes);
+        uint8_t* const to_q = smem + L::kRing + 2 * st * L::kTile;
+        auto load = [&](uint8_t* dst, const CUtensorMap* from, uint64_t* bar) {
 #pragma unroll
-        for (int c = 0; c < NS; ++c) {
-          uint8_t* dst = smem + L::kRing + 2 * st * L::kTile + c * 16384;
-          tma_load_4d(dst, &p.q_map, &q_full[st], c * 64, qt * 128, h, x.w.b);
-          tma_load_4d(dst + L::kTile, &p.do_map, &q_full[st], c * 64, qt * 128, h, x.w.b);
-        }
+          for (int c = 0; c < NS; ++c) tma_load_4d(dst + c * 16384, from, bar, c * 64, qt * 128, h, x.w.b);
+        };
+        // dO's place is free after dV, long before Q's is: what is loaded late is half as much
+        if (use > 0 && !band_wait(&do_empty[st], (use - 1) & 1, abort_flag, a.status, 104)) break;
+        mbar_expect_tx(&do_full[st], L::kTile);
+        load(to_q + L::kTile, &p.do_map, &do_full[st]);
+        if (use > 0 && !band_wait(&q_empty[st], (use - 1) & 1, abort_flag, a.status, 102)) break;
+        mbar_expect_tx(&q_full[st], L::kTile + stat_bytes);
+        load(to_q, &p.q_map, &q_full[st]);
         bulk_load(smem + L::kStat + st * kStatBlock * 4,
                   p.stat + ((static_cast<long long>(x.w.b) * a.Hq + h) * p.n_qt + qt) * kStatBlock, stat_bytes, &q_full[st]);
       }
     } else if (warp >= kMmaWarp && warp < kMmaWarp + G::kGroups) {
       // -------------------------------------------------------- MMA issuer --
-      // In order, for step n: dV with P^T, then S^T of the next step in its place; dK with dS^T, then dP^T of the next step.
-      // The tensor core has the products of one operand to work on while the compute warps make the other.
+      // For step n: dV with P^T, then S^T of the next step in its place; dK with dS^T, then dP^T of the next step.  The tensor
+      // core has the products of one operand to work on while the compute warps make the other.  Where there is room for two
+      // query tiles only, the next but one is loaded into this one's place after dK: dK goes before S^T when it can.
       constexpr uint32_t idesc_s = make_idesc_bf16(128, G::kWidth, false, false);
       constexpr uint32_t idesc_d = make_idesc_bf16(128, D, false, true);
       const int g = warp - kMmaWarp;
@@ -1716,6 +1750,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
       uint32_t n = 0, n_item = 0;  // step, item of `x`
       bool more = x.open(p, 0);
       auto q_bar = [&](uint32_t i) { return BandBar{&q_full[i % ST], (i / ST) & 1}; };
+      auto do_bar = [&](uint32_t i) { return BandBar{&do_full[i % ST], (i / ST) & 1}; };
       auto scores = [&](uint32_t i, uint32_t item) {
         if (one) {
           mma_scores<D>(t_s, desc_k(kv + 2 * (item % KS) * L::kTile), desc_k(ring + 2 * (i % ST) * L::kTile), idesc_s);
@@ -1729,7 +1764,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
           if (last) tc_commit(&kv_empty[item % KS]);
         }
       };
-      bool ok = more && band_wait_all(abort_flag, a.status, 103, BandBar{&kv_full[0], 0}, q_bar(0));
+      bool ok = more && band_wait_all(abort_flag, a.status, 103, BandBar{&kv_full[0], 0}, q_bar(0), do_bar(0));
       if (ok) {
         tc_fence_after();
         scores(0, 0);
@@ -1743,22 +1778,38 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
         if (x_first && n_item > 0 && !band_wait(acc_empty, (n_item - 1) & 1, abort_flag, a.status, 108)) break;
         if (!band_wait(&p_full[g], n & 1, abort_flag, a.status, 109)) break;
         tc_fence_after();
-        if (one) mma_apply<G::kWidth / 16, 2, 32>(t_dv, t_s, desc_mn(sq + L::kTile), idesc_d, x_first);
-        if (ahead) {  // looked for while dV runs
-          const BandBar k_bar{&kv_full[n_item2 % KS], (n_item2 / KS) & 1};
-          ok = fresh ? band_wait_all(abort_flag, a.status, 106, k_bar, q_bar(n + 1))
-                     : band_wait(q_bar(n + 1).bar, q_bar(n + 1).parity, abort_flag, a.status, 106);
-          if (!ok) break;
-          scores(n + 1, n_item2);
+        if (one) {
+          mma_apply<G::kWidth / 16, 2, 32>(t_dv, t_s, desc_mn(sq + L::kTile), idesc_d, x_first);
+          tc_commit(&do_empty[n % ST]);
         }
-        if (!band_wait(&ds_full[g], n & 1, abort_flag, a.status, 111)) break;
+        const BandBar ds_bar{&ds_full[g], n & 1}, k_bar{&kv_full[n_item2 % KS], (n_item2 / KS) & 1};
+        const int late = !ahead  ? 0
+                         : fresh ? band_wait_first(abort_flag, a.status, 106, ds_bar, k_bar, q_bar(n + 1))
+                                 : band_wait_first(abort_flag, a.status, 106, ds_bar, q_bar(n + 1));
+        if (late == 2) break;
+        if (late == 0) {
+          if (ahead) {
+            tc_fence_after();
+            scores(n + 1, n_item2);
+          }
+          if (!band_wait(ds_bar.bar, ds_bar.parity, abort_flag, a.status, 111)) break;
+        }
         tc_fence_after();
         if (one) {
           mma_apply<G::kWidth / 16, 2, 32>(t_dk, t_s + kDp, desc_mn(sq), idesc_d, x_first);
           tc_commit(&q_empty[n % ST]);
           if (x_last) tc_commit(&acc_full[g]);
         }
-        if (ahead) dps(n + 1, n_item2, y_last);
+        if (ahead) {
+          if (late == 1) {
+            if (!band_wait_all(abort_flag, a.status, 107, k_bar, q_bar(n + 1))) break;
+            tc_fence_after();
+            scores(n + 1, n_item2);
+          }
+          if (!band_wait(do_bar(n + 1).bar, do_bar(n + 1).parity, abort_flag, a.status, 105)) break;
+          tc_fence_after();
+          dps(n + 1, n_item2, y_last);
+        }
         x = y;
         more = ahead;
         n_item = n_item2;
@@ -1782,6 +1833,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
       const int item = item_of_round(round);
       if (item >= p.n_items) continue;
       const DkvItem w = dkv_item(p, item);
+      if (w.slot >= 0 && w.per_head == 0) continue;  // no row sees the tile, and none reads its pieces
       const int j = w.kv0 + r;
       int lut_h = -1;
       float far_bias = 0.f;
@@ -1811,7 +1863,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
         const float* stat = reinterpret_cast<const float*>(smem + L::kStat) + st * kStatBlock + quarter * 32;
         const bool added = a.table != nullptr && (pmin - (w.kv0 + 127) < p.t_last || fabsf(far_bias) > 1e30f);
         const bool whole = w.kv0 + 127 <= pmin && w.kv0 + 127 < a.Skv && (pmin + 127 - w.kv0 < a.window || w.kv0 + 127 < a.sinks);
-        if (whole && !added && qt * 128 + 128 <= a.Sq) {  // as in the dQ kernel
+        if (!added && qt * 128 + 128 <= a.Sq) {  // as in the dQ kernel
           exps32<true>(s, pack2(sl2, sl2), stat);
         } else if (!added) {
           exps32<false>(s, pack2(sl2, sl2), stat);
@@ -1944,6 +1996,13 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dkv_kernel(const __g
   }
 }
 
+// Steps (query tiles times heads) of a key tile, as in dkv_item.
+__host__ __device__ __forceinline__ int dkv_steps(const BandArgs& a, int tile) {
+  const int kv0 = tile * 128, first = max(0, kv0 - a.q_pos0);
+  const int last = kv0 < a.sinks ? a.Sq - 1 : min(a.Sq - 1, min(kv0 + 127, a.Skv - 1) - a.q_pos0 + a.window - 1);
+  return first <= last ? ((last >> 7) - (first >> 7) + 1) * (a.Hq / a.Hkv) : 0;
+}
+
 // What is left after them, in one launch.  The first `sum_blocks` blocks add the pieces of split key tiles, in order: eight
 // values of a row per thread.  The others add the table's gradient, over batches and query tiles in a fixed order: a warp per
 // (head, bucket).
@@ -1980,14 +2039,14 @@ __global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant_
   idx /= 128;
   const int which = idx % 2;
   idx /= 2;
-  const int hb = idx % n_hb, tile = first + static_cast<int>(idx / n_hb);
-  if (tile >= end) return;
-  const int j = tile * 128 + r;
+  const int hb = idx % n_hb, nth = first + static_cast<int>(idx / n_hb);
+  if (nth >= end) return;
+  const bool sink = nth < p.sink_tiles;
+  const int j = (sink ? nth : other_tile(p, nth - p.sink_tiles)) * 128 + r;
   if (j >= a.Skv) return;
-  const bool sink = tile < p.sink_tiles;
-  const int pieces = sink ? p.sink_pieces : p.pieces;
-  const int slot0 = sink ? tile * pieces * n_hb + hb
-                         : (p.sink_pieces > 1 ? sink_items : 0) + (tile - p.sink_tiles) * pieces * n_hb + hb;
+  const int pieces = dkv_steps(a, j >> 7) == 0 ? 0 : sink ? p.sink_pieces : p.pieces;
+  const int slot0 = sink ? nth * pieces * n_hb + hb
+                         : (p.sink_pieces > 1 ? sink_items : 0) + (nth - p.sink_tiles) * pieces * n_hb + hb;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < pieces; ++i) {
     const float4* src = reinterpret_cast<const float4*>(
@@ -2003,17 +2062,11 @@ __global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant_
                                               pack_bf16x2(x[4] * mul, x[5] * mul), pack_bf16x2(x[6] * mul, x[7] * mul));
 }
 
-// Steps (query tiles times heads) of a key tile, as in dkv_item.
-static int dkv_steps(const BandArgs& a, int tile) {
-  const int kv0 = tile * 128, first = std::max(0, kv0 - a.q_pos0);
-  const int last = kv0 < a.sinks ? a.Sq - 1 : std::min(a.Sq - 1, std::min(kv0 + 127, a.Skv - 1) - a.q_pos0 + a.window - 1);
-  return first <= last ? ((last >> 7) - (first >> 7) + 1) * (a.Hq / a.Hkv) : 0;
-}
-
 // Into how many pieces the steps of a key tile are cut.  Cutting costs the pieces' way through memory and a launch; not
 // cutting leaves SMs idle when there are few key tiles and heads (grouped heads), or when the tiles that hold sinks, which
 // every query sees, take many times as long as the others.  The estimate, in steps: the sum over rounds of the longest item
-// of each, with two steps for an item's beginning and end, one more for a piece and two for the launch that adds them up.
+// of each, with two steps for an item's beginning and end, four more for a piece (writing 128 KB of fp32 sums took as long as
+// 2.6 steps at D = 128, and they are read again) and two for the launch that adds them up.
 static void plan_pieces(BandBwdParams& p) {
   const BandArgs& a = p.a;
   const int sms = sm_count(), n_hb = a.Hkv * a.B;
@@ -2024,6 +2077,7 @@ static void plan_pieces(BandBwdParams& p) {
     most = std::max(most, dkv_steps(a, t));
   }
   const int others = p.n_kt - p.sink_tiles;
+  p.first_seen = std::min(std::max(p.sink_tiles, std::max(0, a.q_pos0 - a.window + 1) >> 7), p.n_kt - (others > 0));
   double best = 1e30;
   for (int c : {1, 2, 3, 4, 6, 8, 12, 16}) {
     if (c > longest || (c > 1 && others == 0)) break;
@@ -2034,8 +2088,9 @@ static void plan_pieces(BandBwdParams& p) {
       const long long items = sink_items + static_cast<long long>(others) * c * n_hb;
       double cost = (c > 1 || cs > 1) ? 2.0 : 0.0;
       for (long long i = 0; i < items; i += sms) {
-        if (i < sink_items) cost += (longest_sink + cs - 1) / cs + (cs > 1 ? 3 : 2);
-        else cost += (dkv_steps(a, p.sink_tiles + static_cast<int>((i - sink_items) / n_hb / c)) + c - 1) / c + (c > 1 ? 3 : 2);
+        if (i < sink_items) cost += (longest_sink + cs - 1) / cs + (cs > 1 ? 6 : 2);
+        else if (const int steps = dkv_steps(a, other_tile(p, static_cast<int>((i - sink_items) / n_hb / c))))
+          cost += (steps + c - 1) / c + (c > 1 ? 6 : 2);
       }
       if (cost < best) {
         best = cost;
