@@ -1036,21 +1036,32 @@ struct BandBwdParams {
 // A block per query tile; D / 8 lanes a row (16 bytes each of dO, O and what was cut off of it), a thread's rows in flight together.
 // In the dQ kernel, a thread per quarter row, the same loads hit a line per lane and cost an item 4000 clocks.
 template <int D>
-__global__ void __launch_bounds__(256, 2) band_stat_kernel(const __grid_constant__ BandBwdParams p) {
+__host__ __device__ constexpr int stat_blocks() { return D == 64 ? 1 : 2; }
+template <int D>
+__global__ void __launch_bounds__(256, 3) band_stat_kernel(const __grid_constant__ BandBwdParams p) {
   pdl_enter();
   const BandArgs& a = p.a;
   constexpr int kLanes = D == 64 ? 8 : 16;  // 12 of 16 at D = 96
-  constexpr int kRowsAtOnce = 256 / kLanes, kStatRows = 128 / kRowsAtOnce;
+  constexpr int kRowsAtOnce = 256 / kLanes, kStatRows = 4, kParts = stat_blocks<D>();
   const int sub = threadIdx.x / kLanes, part = threadIdx.x % kLanes;
   // heads run fastest: their rows lie next to one another in memory
   int rest_of, h;
-  const int qt = p.by_hqb.quot(static_cast<int>(blockIdx.x), rest_of), b = p.by_hq.quot(rest_of, h);
+  const int at_qt = p.by_hqb.quot(static_cast<int>(blockIdx.x), rest_of), b = p.by_hq.quot(rest_of, h);
+  const int qt = at_qt / kParts, r0 = at_qt % kParts * (kRowsAtOnce * kStatRows) + sub;
   const long long tile = (static_cast<long long>(b) * a.Hq + h) * p.n_qt + qt;
   const bool mine = part * 8 < D;
   uint4 o[kStatRows], rest[kStatRows], g[kStatRows];
+  float m[kStatRows], l[kStatRows];
 #pragma unroll
   for (int i = 0; i < kStatRows; ++i) {
-    const int row = qt * 128 + i * kRowsAtOnce + sub;
+    const int row = qt * 128 + r0 + i * kRowsAtOnce;
+    m[i] = INFINITY;
+    l[i] = 0.f;
+    if (part == 0 && row < a.Sq) {
+      const long long at = (static_cast<long long>(b) * a.Hq + h) * a.Sq + row;
+      m[i] = a.m[at];
+      l[i] = a.l[at];
+    }
     if (mine && row < a.Sq) {
       o[i] = *reinterpret_cast<const uint4*>(band_row(a.o, a.o_st, b, row, h) + part * 8);
       rest[i] = row < a.rest_rows ? *reinterpret_cast<const uint4*>(rest_row(a, b, row, h, D) + part * 8) : make_uint4(0, 0, 0, 0);
@@ -1073,14 +1084,12 @@ __global__ void __launch_bounds__(256, 2) band_stat_kernel(const __grid_constant
     }
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    const int r = i * kRowsAtOnce + sub, row = qt * 128 + r;
+    const int r = r0 + i * kRowsAtOnce;
     if (part == 0) {
-      const long long at = (static_cast<long long>(b) * a.Hq + h) * a.Sq + row;
-      const float m = row < a.Sq ? a.m[at] : INFINITY, l = row < a.Sq ? a.l[at] : 0.f;
-      st[r] = (far_bias - m) - l;
+      st[r] = (far_bias - m[i]) - l[i];
       st[128 + r] = sum;
-      st[256 + r] = m;
-      st[384 + r] = l;
+      st[256 + r] = m[i];
+      st[384 + r] = l[i];
     }
   }
 }
@@ -2131,7 +2140,7 @@ static BandScratch plan_bwd(BandBwdParams& p, const BandArgs& a) {
 template <int D>
 static cudaError_t launch_band_bwd(BandBwdParams& p, long long dq_items, long long dkv_items, bool split, cudaStream_t s) {
   const int lut = p.a.table == nullptr ? 0 : lut_bytes(p.t_last, 1);
-  cudaError_t e = launch_pdl(band_stat_kernel<D>, dim3(static_cast<unsigned>(dq_items)), dim3(256), 0, s, p);
+  cudaError_t e = launch_pdl(band_stat_kernel<D>, dim3(static_cast<unsigned>(dq_items * stat_blocks<D>())), dim3(256), 0, s, p);
   if (e != cudaSuccess) return e;
   p.n_items = static_cast<int>(dq_items);
   e = launch_pdl(band_bwd_dq_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads),
