@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 
 namespace nmb {
 
@@ -2073,12 +2074,14 @@ __global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant_
 
 // Into how many pieces the steps of a key tile are cut.  Cutting costs the pieces' way through memory and a launch; not
 // cutting leaves SMs idle when there are few key tiles and heads (grouped heads), or when the tiles that hold sinks, which
-// every query sees, take many times as long as the others.  The estimate, in steps: the sum over rounds of the longest item
-// of each, with two steps for an item's beginning and end, four more for a piece (writing 128 KB of fp32 sums took as long as
-// 2.6 steps at D = 128, and they are read again) and two for the launch that adds them up.
+// every query sees, take many times as long as the others.  The estimate, in steps: what the most loaded of five of the SMs
+// gets, with two steps for an item's beginning and end, D / 32 more for a piece (writing 128 KB of fp32 sums took as long
+// as 2.6 steps at D = 128, and they are read again) and two for the launch that adds them up.  Over 300 shapes its choice was
+// 0.4 percent behind the best one of all SMs' loads, never cutting 58 percent.
 static void plan_pieces(BandBwdParams& p) {
   const BandArgs& a = p.a;
-  const int sms = sm_count(), n_hb = a.Hkv * a.B;
+  const int sms = sm_count(), n_hb = a.Hkv * a.B, piece_cost = 2 + a.d / 32;
+  constexpr int kMaxRounds = 16;  // those after them are alike, and cutting gains nothing where there are as many
   p.sink_tiles = a.window >= a.q_pos0 + a.Sq ? 0 : std::min((std::min(a.sinks, a.Skv) + 127) / 128, p.n_kt);
   int longest = 1, longest_sink = 1;
   for (int t = 0; t < p.n_kt; ++t) {
@@ -2087,25 +2090,36 @@ static void plan_pieces(BandBwdParams& p) {
   }
   const int others = p.n_kt - p.sink_tiles;
   p.first_seen = std::min(std::max(p.sink_tiles, std::max(0, a.q_pos0 - a.window + 1) >> 7), p.n_kt - (others > 0));
-  double best = 1e30;
+  p.pieces = p.sink_pieces = 1;
+  int best = INT_MAX;
   for (int c : {1, 2, 3, 4, 6, 8, 12, 16}) {
-    if (c > longest || (c > 1 && others == 0)) break;
+    if (c > 1 && (c > longest || static_cast<long long>(others) * c * n_hb > static_cast<long long>(kMaxRounds) * sms)) break;
     const int piece = (longest + c - 1) / c;
     const int even = p.sink_tiles == 0 ? 1 : std::min(64, (longest_sink + std::max(piece, 4) - 1) / std::max(piece, 4));
     for (int cs : {1, even}) {
       const long long sink_items = static_cast<long long>(p.sink_tiles) * cs * n_hb;
       const long long items = sink_items + static_cast<long long>(others) * c * n_hb;
-      double cost = (c > 1 || cs > 1) ? 2.0 : 0.0;
-      for (long long i = 0; i < items; i += sms) {
-        if (i < sink_items) cost += (longest_sink + cs - 1) / cs + (cs > 1 ? 6 : 2);
-        else if (const int steps = dkv_steps(a, other_tile(p, static_cast<int>((i - sink_items) / n_hb / c))))
-          cost += (steps + c - 1) / c + (c > 1 ? 6 : 2);
+      const int rounds = static_cast<int>(std::min<long long>((items + sms - 1) / sms, kMaxRounds));
+      int cost = 0;
+      for (int part = 0; part < 5; ++part) {
+        const int sm = part * (sms - 1) / 4;
+        int load = 0;
+        for (int round = 0; round < rounds; ++round) {
+          const long long i = static_cast<long long>(round) * sms + ((round & 1) ? sms - 1 - sm : sm);
+          if (i >= items) break;
+          if (i < sink_items) load += (longest_sink + cs - 1) / cs + (cs > 1 ? piece_cost : 2);
+          else if (const int steps = dkv_steps(a, other_tile(p, static_cast<int>((i - sink_items) / n_hb / c))))
+            load += (steps + c - 1) / c + (c > 1 ? piece_cost : 2);
+        }
+        cost = std::max(cost, load);
       }
+      if (c > 1 || (cs > 1 && p.sink_tiles > 0)) cost += 2;
       if (cost < best) {
         best = cost;
         p.pieces = c;
         p.sink_pieces = cs;
       }
+      if (even == 1) break;
     }
   }
 }
