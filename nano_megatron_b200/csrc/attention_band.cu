@@ -239,10 +239,7 @@ __device__ __forceinline__ void exp2_pair_fma(uint64_t x2, float& y0, float& y1)
   y1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
 // One pair in this many takes that way.
-#ifndef NMB_FMA_PAIRS
-#define NMB_FMA_PAIRS 4
-#endif
-constexpr int kFmaPairs = NMB_FMA_PAIRS;
+constexpr int kFmaPairs = 4;
 template <bool kMix>
 __device__ __forceinline__ void exp2_pair(int pair, uint64_t x2, float& y0, float& y1) {
   if (kMix && (pair % kFmaPairs) == kFmaPairs - 1) {
@@ -506,7 +503,7 @@ __device__ __forceinline__ FwdItem fwd_item(const BandFwdParams& p, int item) {
   return w;
 }
 
-template <int D>
+template <int D, bool kExact>
 __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_constant__ BandFwdParams p) {
   using L = BandFwdSmem<D>;
   constexpr int NS = L::kSlabs, ST = L::kStages;
@@ -522,7 +519,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
   uint64_t* p_full = q_full + 6;
   uint64_t* o_full = q_full + 8;
   uint64_t* o_empty = q_full + 10;
-  uint64_t* s_read = q_full + 12;        // only with P's own columns, as the next
+  uint64_t* s_read = q_full + 12;        // only with P's own columns
   uint64_t* pv_done = q_full + 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -650,21 +647,26 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
           const uint32_t pos = base + 2 * u;
           return BandBar{&kv_full[pos % ST], (pos / ST) & 1};
         };
-        // O += P V of tile u, whose V is there
+        auto p_bar = [&](int i) { return BandBar{&p_full[t0 + i], n_p[i] & 1}; };
+        // O += P V of tile u, whose V and P are there
         auto pv = [&](int i, int u, bool last) {
           const int t = t0 + i;
-          tc_fence_after();
-          if (one) {
-            const uint32_t b_low = desc_mn(ring + ((base + 2 * u + 1) % ST) * L::kTile);
-            mma_apply<8, kOwn ? 8 : 4, 64>(tmem + 256 + t * D, tmem + (kOwn ? 384 + t * 64 : t * 128), b_low, idesc_o, first_pv[i]);
-            if (kOwn) tc_commit(&pv_done[t]);
-            if (last) tc_commit(&o_full[t]);
+          const uint32_t b_low = desc_mn(ring + ((base + 2 * u + 1) % ST) * L::kTile);
+#pragma unroll
+          for (int part = 0; part < (kExact ? 2 : 1); ++part) {  // the weights, then what was cut off of them
+            if (part == 1 && !band_wait(p_bar(i).bar, p_bar(i).parity, abort_flag, a.status, 77)) return false;
+            tc_fence_after();
+            if (one) {
+              mma_apply<8, kOwn ? 8 : 4, 64>(tmem + 256 + t * D, tmem + (kOwn ? 384 + t * 64 : t * 128), b_low, idesc_o, first_pv[i]);
+              if (kOwn || kExact) tc_commit(&pv_done[t]);
+              if (last && (!kExact || part == 1)) tc_commit(&o_full[t]);
+            }
+            ++n_p[i];
+            first_pv[i] = false;
           }
-          ++n_p[i];
-          first_pv[i] = false;
           pending[i] = false;
+          return true;
         };
-        auto p_bar = [&](int i) { return BandBar{&p_full[t0 + i], n_p[i] & 1}; };
         auto o_free = [&](int i) {  // the accumulator, for the first product of an item
           return !first_pv[i] || n_item[i] == 0 || band_wait(&o_empty[t0 + i], (n_item[i] - 1) & 1, abort_flag, a.status, 64);
         };
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
             if (ok) release(base + 2 * u);
             if (ok && was) {
               ok = o_free(0) && band_wait_all(abort_flag, a.status, 63, v_bar(u - 1), p_bar(0));
-              if (ok) pv(0, u - 1, left[0] == 0 && !use);
+              ok = ok && pv(0, u - 1, left[0] == 0 && !use);
             }
             if (ok && u > 0) {  // V of a tile that only the other slot works on: passed on once it is there, not before
               if (!was) ok = band_wait(v_bar(u - 1).bar, v_bar(u - 1).parity, abort_flag, a.status, 76);
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
                 ok = o_free(i) && (k_there && v_there ? band_wait(p_bar(i).bar, p_bar(i).parity, abort_flag, a.status, 65)
                                                       : band_wait_all(abort_flag, a.status, 65, k_bar(u), v_bar(u - 1), p_bar(i)));
                 k_there = v_there = true;
-                if (ok) pv(i, u - 1, left[i] == 0);
+                ok = ok && pv(i, u - 1, left[i] == 0);
               }
               if (ok && use) {
                 ok = (k_there || band_wait(k_bar(u).bar, k_bar(u).parity, abort_flag, a.status, 66)) && scores(i, u);
@@ -736,7 +738,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
           if (ok && pending[i]) {
             ok = o_free(i) && band_wait_all(abort_flag, a.status, 65, v_bar(n - 1), p_bar(i));
             v_there = true;
-            if (ok) pv(i, n - 1, true);
+            ok = ok && pv(i, n - 1, true);
           }
         }
         if (ok && n > 0) {
@@ -759,7 +761,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
     const float sl2 = a.scale * kBandLog2e;
     float* lut = luts + t * entries;
     float* xch = reinterpret_cast<float*>(smem + L::kXch) + t * 256 + r;
-    int n_s = 0, n_item = 0, parity = 0;
+    int n_s = 0, n_pv = 0, n_item = 0, parity = 0;
     bool ok = true;
     // the other thread's value of this row
     auto other = [&](float mine) {
@@ -853,7 +855,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         const float alpha = m_new == m ? 1.f : ex2(m - m_new);  // m == -inf: 0
         const float shift = add - (m_new == -INFINITY ? 0.f : m_new);
         // The product of the tile before is done: with shared columns the scores came after it.
-        if (kOwn && n_s > 1) NMB_BAND_WAIT(&pv_done[t], n_s & 1, 73);
+        if (kOwn && n_pv > 0) NMB_BAND_WAIT(&pv_done[t], (n_pv - 1) & 1, 73);
         if (u > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
           tc_fence_after();
 #pragma unroll 1
@@ -868,23 +870,52 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         }
         const uint64_t mul_2 = pack2(mul, mul), shift_2 = pack2(shift, shift);
         uint64_t sum = pack2(0.f, 0.f);
+        auto pass_on = [&]() {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+          ++n_pv;
+        };
+        if constexpr (!kExact) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
-          if (part[c] == 2) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
+            if (part[c] == 2) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) pk[k] = 0;
-          } else if (part[c] == 1 && !added) {
-            weights32<true>(s[c], mul_2, shift_2, sum, pk);
-          } else {
-            weights32<false>(s[c], mul_2, shift_2, sum, pk);
+              for (int k = 0; k < 16; ++k) pk[k] = 0;
+            } else if (part[c] == 1 && !added) {
+              weights32<true>(s[c], mul_2, shift_2, sum, pk);
+            } else {
+              weights32<false>(s[c], mul_2, shift_2, sum, pk);
+            }
+            tmem_st_32x16(t_p + c * 16, pk);
           }
-          tmem_st_32x16(t_p + c * 16, pk);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float p0 = 0.f, p1 = 0.f;
+              if (part[c] != 2) {
+                unpack2(fma2(pack2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), mul_2, shift_2), p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+              }
+              sum = add2(sum, pack2(p0, p1));
+              pk[k] = pack_bf16x2(p0, p1);
+              s[c][k] = pack_bf16x2(p0 - __uint_as_float(pk[k] << 16), p1 - __uint_as_float(pk[k] & 0xffff0000u));
+            }
+            tmem_st_32x16(t_p + c * 16, pk);
+          }
+          pass_on();
+          NMB_BAND_WAIT(&pv_done[t], (n_pv - 1) & 1, 78);
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tmem_st_32x16(t_p + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(s[c]));
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        pass_on();
         float sum0, sum1;
         unpack2(sum, sum0, sum1);
         l = l * alpha + (sum0 + sum1);
@@ -976,10 +1007,20 @@ static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStr
   return make_tmap_bf16(m, ptr, 4, dims, strides, box);
 }
 
+// With kExact the weights go into O to twice bf16's digits, the head and what it cut off in two products one after the other.
+// A bias table's gradient is a sum over dS in which O's error does not cancel: with bf16 weights it was 2.2 times as far from
+// the exact one as its own rounding at 22 keys, 1.4 times at most above 512 keys, where the errors average out; with both it is
+// no further at any.  So training with a table pays for the second product up to kExactKeys keys a row (8 x 512 rows, 16
+// heads, D = 64, window 128: 20 -> 27 us) and nothing else does.  A variant of its own: the test inside the loop cost the
+// others 10 percent through registers.
+constexpr int kExactKeys = 512;
 template <int D>
 static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
-  const int lut = p.a.table == nullptr ? 0 : lut_bytes(p.t_last, 2);
-  return launch_pdl(band_fwd_kernel<D>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
+  const BandArgs& a = p.a;
+  const int lut = a.table == nullptr ? 0 : lut_bytes(p.t_last, 2);
+  const bool exact = a.table != nullptr && a.rest_rows > 0 &&
+                     std::min<long long>(a.Skv, static_cast<long long>(a.window) + a.sinks) <= kExactKeys;
+  return launch_pdl(exact ? band_fwd_kernel<D, true> : band_fwd_kernel<D, false>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
 }
 
 // --------------------------------------------------------------- backward --
@@ -2213,9 +2254,12 @@ extern "C" int nmb_band_configure() {
       e = cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   };
   const int lut = lut_bytes(kMaxDistance, 2);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64>), BandFwdSmem<64>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96>), BandFwdSmem<96>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128>), BandFwdSmem<128>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, false>), BandFwdSmem<64>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, true>), BandFwdSmem<64>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, false>), BandFwdSmem<96>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, true>), BandFwdSmem<96>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, false>), BandFwdSmem<128>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, true>), BandFwdSmem<128>::kLut + lut);
   const int lut1 = lut_bytes(kMaxDistance, 1);
   opt_in(reinterpret_cast<const void*>(band_bwd_dq_kernel<64>), BandDqSmem<64>::kLut + lut1 + BandDqSmem<64>::kBins);
   opt_in(reinterpret_cast<const void*>(band_bwd_dq_kernel<96>), BandDqSmem<96>::kLut + lut1 + BandDqSmem<96>::kBins);

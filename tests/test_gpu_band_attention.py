@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from tests._band_oracle import check, oracle
+from tests._band_oracle import bucket, check, oracle, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -348,3 +348,29 @@ def test_not_differentiable_twice():
     assert all(torch.equal(a, b) for a, b in zip(grads, plain))
     with pytest.raises(RuntimeError, match="differentiated again"):
         grads[0].float().square().sum().backward()
+
+
+@pytest.mark.parametrize("sq,hq,hkv,d,window,buckets,max_distance", [
+    (3, 8, 1, 64, None, 18, 43), (22, 8, 1, 64, 21, 3, 27), (344, 4, 1, 128, None, 30, 43), (512, 2, 2, 96, None, 32, 128),
+    (700, 2, 1, 64, 130, 4, 60)])
+def test_gradient_of_the_bias_over_few_keys(sq, hq, hkv, d, window, buckets, max_distance):
+    """Where a row sees few keys the table's gradient is as exact as fp32 sums of D's error allow: D comes from weights of
+    twice bf16's digits, the output and what its rounding cut off: 2^-17 and 2^-18 of sum_j P_j sum_d |dO V_j|; the rest is held in
+    fp32: 2^-17 of the terms for scores, exponentials and sums."""
+    q, k, v, table, dout = _tensors(2, sq, sq, hq, hkv, d, buckets, table_dtype=torch.float32)
+    out = _call(q, k, v, table, d ** -0.5, max_distance, window=window)
+    got = torch.autograd.grad(out, (q, k, v, table), dout)[3]
+    values, _, _ = oracle(q, k, v, dout, d ** -0.5, window=window, table=table, max_distance=max_distance)
+    g, kh, vh = dout.double().transpose(1, 2), k.detach().double().transpose(1, 2), v.detach().double().transpose(1, 2)
+    kh, vh = (t.repeat_interleave(hq // hkv, 1) for t in (kh, vh))
+    at = (torch.arange(sq)[:, None] - torch.arange(sq)[None, :]).clamp(min=0)
+    at = torch.tensor([bucket(n, buckets, max_distance) for n in range(sq)])[at].cuda()
+    see = visible(sq, sq, window, 0, 0, "cuda")
+    x = (q.detach().double().transpose(1, 2) @ kh.transpose(2, 3)) * d ** -0.5 + table.detach().double()[:, at]
+    p = torch.softmax(x.masked_fill(~see, -math.inf), -1)
+    size = g.abs() @ vh.abs().transpose(2, 3)              # of dP's sums
+    per_row = (p * size).sum(-1, keepdim=True)             # of D's
+    terms = p * (2.0 ** -16 * per_row + 2.0 ** -17 * (size + per_row))
+    bound = torch.zeros_like(values["dtable"]).index_add_(1, at.flatten(), terms.sum(0).flatten(1))
+    assert ((got.double() - values["dtable"]).abs() <= bound + 1e-30).all(), \
+        f"{((got.double() - values['dtable']).abs() / (bound + 1e-30)).max().item():.2f} times what is allowed"
