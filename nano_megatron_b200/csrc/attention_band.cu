@@ -2123,14 +2123,12 @@ static void plan_pieces(BandBwdParams& p) {
   const BandArgs& a = p.a;
   const int sms = sm_count(), n_hb = a.Hkv * a.B, piece_cost = 2 + a.d / 32;
   constexpr int kMaxRounds = 16;  // those after them are alike, and cutting gains nothing where there are as many
-  p.sink_tiles = a.window >= a.q_pos0 + a.Sq ? 0 : std::min((std::min(a.sinks, a.Skv) + 127) / 128, p.n_kt);
   int longest = 1, longest_sink = 1;
   for (int t = 0; t < p.n_kt; ++t) {
     int& most = t < p.sink_tiles ? longest_sink : longest;
     most = std::max(most, dkv_steps(a, t));
   }
   const int others = p.n_kt - p.sink_tiles;
-  p.first_seen = std::min(std::max(p.sink_tiles, std::max(0, a.q_pos0 - a.window + 1) >> 7), p.n_kt - (others > 0));
   p.pieces = p.sink_pieces = 1;
   int best = INT_MAX;
   for (int c : {1, 2, 3, 4, 6, 8, 12, 16}) {
@@ -2168,12 +2166,19 @@ static void plan_pieces(BandBwdParams& p) {
 struct BandScratch {
   long long stat, part, dtable, total;  // floats
 };
-static BandScratch plan_bwd(BandBwdParams& p, const BandArgs& a) {
+static BandScratch plan_bwd(BandBwdParams& p, const BandArgs& a, const BandPlan* plan = nullptr) {
   p.a = a;
   p.n_qt = (a.Sq + 127) / 128;
   p.n_kt = (a.Skv + 127) / 128;
   p.t_last = a.buckets < 2 ? 0 : a.limit[a.buckets - 2];
-  plan_pieces(p);
+  p.sink_tiles = a.window >= a.q_pos0 + a.Sq ? 0 : std::min((std::min(a.sinks, a.Skv) + 127) / 128, p.n_kt);
+  p.first_seen = std::min(std::max(p.sink_tiles, std::max(0, a.q_pos0 - a.window + 1) >> 7), p.n_kt - (p.n_kt > p.sink_tiles));
+  if (plan == nullptr) {
+    plan_pieces(p);
+  } else {
+    p.sink_pieces = plan->sink_pieces;
+    p.pieces = plan->pieces;
+  }
   p.by_hqb = FastDiv(a.Hq * a.B);
   p.by_hq = FastDiv(a.Hq);
   p.by_group = FastDiv(a.Hq / a.Hkv);
@@ -2302,11 +2307,26 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   return e == cudaSuccess ? 0 : 400 + e;
 }
 
+extern "C" int nmb_band_bwd_plan(const BandArgs* a, BandPlan* plan) {
+  if (int bad = band_check(a)) return bad;
+  BandBwdParams p;
+  plan->scratch = plan_bwd(p, *a).total;
+  plan->sink_pieces = p.sink_pieces;
+  plan->pieces = p.pieces;
+  return 0;
+}
+
 extern "C" int nmb_band_bwd(const BandArgs* a, void* stream) {
+  BandPlan plan;
+  if (int bad = nmb_band_bwd_plan(a, &plan)) return bad;
+  return nmb_band_bwd_planned(a, &plan, stream);
+}
+
+extern "C" int nmb_band_bwd_planned(const BandArgs* a, const BandPlan* plan, void* stream) {
   if (int bad = band_check(a)) return bad;
   (void)cudaGetLastError();
   BandBwdParams p;
-  const BandScratch w = plan_bwd(p, *a);
+  const BandScratch w = plan_bwd(p, *a, plan);
   p.stat = a->scratch;
   p.part = p.stat + w.stat;
   p.dtable_part = p.part + w.part;

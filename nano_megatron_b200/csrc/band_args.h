@@ -33,6 +33,12 @@ struct BandArgs {
   unsigned short limit[kMaxBuckets];  // first distance of bucket b + 1
 };
 
+// How the backward pass cuts key tiles that take long, and what it needs for that; of the sizes alone.
+struct BandPlan {
+  int sink_pieces, pieces;
+  long long scratch;  // floats
+};
+
 }  // namespace nmb
 
 extern "C" {
@@ -41,6 +47,9 @@ int nmb_band_args_size();
 long long nmb_band_bwd_scratch(const nmb::BandArgs* a);
 int nmb_band_fwd(const nmb::BandArgs* a, void* stream);
 int nmb_band_bwd(const nmb::BandArgs* a, void* stream);
+// The two steps of the backward pass for a caller that makes `scratch` in between.
+int nmb_band_bwd_plan(const nmb::BandArgs* a, nmb::BandPlan* plan);
+int nmb_band_bwd_planned(const nmb::BandArgs* a, const nmb::BandPlan* plan, void* stream);
 // Kernels launched by the two so far.
 long long nmb_band_launches();
 }

@@ -11,6 +11,7 @@
 #include <torch/library.h>
 
 #include <array>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <vector>
@@ -135,8 +136,8 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
     TORCH_CHECK(rc == 0, "nmb_band_fwd: launcher returned ", rc);
     if (train) {
       ctx->save_for_backward({q, k, v, table, out, rest, stats});
-      ctx->saved_data["scale"] = scale;
-      ctx->saved_data["numbers"] = std::vector<int64_t>{window, sinks, start, max_distance};
+      ctx->saved_data["numbers"] =  // all of them exact in a double
+          std::vector<double>{scale, double(window), double(sinks), double(start), double(max_distance)};
     }
     return out;
   }
@@ -160,9 +161,10 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &out = saved[4], &rest = saved[5], &stats = saved[6];
     variable_list result(10);
     const c10::cuda::CUDAGuard guard(q.device());
-    const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
+    const std::vector<double> n = ctx->saved_data["numbers"].toDoubleVector();
     const Tensor dout = dout_in.defined() ? readable(dout_in.is_contiguous() ? dout_in : dout_in.contiguous()) : at::zeros_like(out);
-    nmb::BandArgs a = arguments(q, k, v, table, out, rest, stats, ctx->saved_data["scale"].toDouble(), n[0], n[1], n[2], n[3]);
+    nmb::BandArgs a = arguments(q, k, v, table, out, rest, stats, n[0], static_cast<int64_t>(n[1]),
+                                static_cast<int64_t>(n[2]), static_cast<int64_t>(n[3]), static_cast<int64_t>(n[4]));
     Tensor dq, dk, dv;
     // q, k and v the slices of one packed projection: their gradients go to the slices of one buffer, and are joined
     // without a copy
@@ -189,9 +191,12 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
       a.dtable = result[3].data_ptr();
       a.dtable_fp32 = a.table_fp32;
     }
-    const Tensor scratch = at::empty({nmb_band_bwd_scratch(&a)}, stats.options());
+    nmb::BandPlan plan;
+    const int bad = nmb_band_bwd_plan(&a, &plan);
+    TORCH_CHECK(bad == 0, "nmb_band_bwd_plan: returned ", bad);
+    const Tensor scratch = at::empty({plan.scratch}, stats.options());
     a.scratch = scratch.data_ptr<float>();
-    const int rc = nmb_band_bwd(&a, current_stream(q));
+    const int rc = nmb_band_bwd_planned(&a, &plan, current_stream(q));
     TORCH_CHECK(rc == 0, "nmb_band_bwd: launcher returned ", rc);
     result[0] = dq;
     result[1] = dk;
@@ -200,8 +205,32 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
   }
 };
 
-Tensor band_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& table, double scale, int64_t window,
-                      int64_t sinks, int64_t start, int64_t max_distance) {
+// Is this a call that the kernels take as it is?  All that the entry points in Python look at, for one look from here.
+bool ready(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& table, double scale, int64_t window,
+           int64_t sinks, int64_t start, int64_t max_distance) {
+  constexpr int64_t kMaxPosition = int64_t{1} << 30, kIntMax = (int64_t{1} << 31) - 1;
+  for (const Tensor* t : {&q, &k, &v})
+    if (!t->defined() || !t->is_cuda() || t->layout() != at::kStrided || t->scalar_type() != at::kBFloat16 || t->dim() != 4 ||
+        t->numel() == 0 || t->device() != q.device())
+      return false;
+  const int64_t d = q.size(3);
+  if (k.sizes() != v.sizes() || q.size(0) != k.size(0) || d != k.size(3) || (d != 64 && d != 96 && d != 128) || q.size(2) % k.size(2) != 0)
+    return false;
+  if (!(std::isfinite(scale) && scale > 0.0) || window < 1 || window > kIntMax || sinks < 0 || sinks > kIntMax || start < 0 ||
+      start > kMaxPosition || start + q.size(1) > kMaxPosition || k.size(1) > kMaxPosition || g_status[q.device().index()] == nullptr)
+    return false;
+  if (!table.has_value()) return true;
+  if (!table->defined() || table->dim() != 2 || table->layout() != at::kStrided || table->device() != q.device() ||
+      table->size(0) != q.size(2) || (table->scalar_type() != at::kBFloat16 && table->scalar_type() != at::kFloat))
+    return false;
+  std::lock_guard<std::mutex> lock(g_limits_mutex);
+  return g_limits.count({table->size(1), max_distance}) != 0;  // what is there has passed the checks
+}
+
+// None where the call is not one for the kernels, or not yet.
+std::optional<Tensor> band_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& table, double scale,
+                                     int64_t window, int64_t sinks, int64_t start, int64_t max_distance) {
+  if (!ready(q, k, v, table, scale, window, sinks, start, max_distance)) return std::nullopt;
   const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                     (table.has_value() && table->requires_grad()));
   return BandAttention::apply(q, k, v, table, scale, window, sinks, start, max_distance, train);
@@ -214,6 +243,6 @@ TORCH_LIBRARY(nmb, m) {
   m.def("band_limits(int buckets, int max_distance, int[] limits) -> ()", band_limits);
   m.def(
       "band_attention(Tensor q, Tensor k, Tensor v, Tensor? table, float scale, int window, int sinks, int start, int max_distance) "
-      "-> Tensor",
+      "-> Tensor?",
       band_attention);
 }

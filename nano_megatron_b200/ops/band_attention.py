@@ -72,6 +72,9 @@ def band_attention_supported(t: Tensor) -> bool:
 
 
 # --------------------------------------------------------------- operators --
+_ready = []  # the operator, once a device has been set up
+
+
 @functools.lru_cache(maxsize=None)
 def _operator(device_index: int):
     """The operator of ``csrc/torch_binding.cpp``, ready for a device (whose status word the kernels report to)."""
@@ -79,7 +82,8 @@ def _operator(device_index: int):
     with torch.cuda.device(device_index):
         native.lib()
         ops.band_device(device_index, native.status_word(torch.device("cuda", device_index)).data_ptr())
-    return ops.band_attention.default
+    _ready[:] = [ops.band_attention.default]
+    return _ready[0]
 
 
 @functools.lru_cache(maxsize=None)
@@ -103,6 +107,12 @@ class _ToMainGrad(torch.autograd.Function):
             buffer.add_(grad) if accumulate else buffer.copy_(grad)
             return buffer
         return _deliver_grad(ctx.param, compute)
+
+
+def _trained(table):
+    if table is not None and getattr(table, "main_grad", None) is not None and table.requires_grad and torch.is_grad_enabled():
+        return _ToMainGrad.apply(table)
+    return table
 
 
 # ------------------------------------------------------------------ checks --
@@ -143,12 +153,17 @@ def _check_shapes(q, k, v, floating, buckets, max_distance, scale, start) -> Non
 
 
 def _attend(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor:
+    if _ready and q.is_cuda and type(scale) is float and type(window) is type(sinks) is type(start) is type(max_distance) is int:
+        # one look from C++ in place of those below, which took as long as the rest of a call together
+        out = _ready[0](q, k, v, _trained(table), scale, window, sinks, start, max_distance)
+        if out is not None:
+            return out
     if not q.dtype == k.dtype == v.dtype:
         raise ValueError(f"q, k, v must share a floating type; got {q.dtype}, {k.dtype}, {v.dtype}")
     if not q.device == k.device == v.device:
         raise ValueError(f"q, k, v must be on one device; got {q.device}, {k.device}, {v.device}")
     if type(window) is not int or type(sinks) is not int or type(start) is not int or window < 1 or sinks < 0 or start < 0:
-        window = _INT_MAX if window is None else _check_int("window", window, 1)
+        window = _check_int("window", window, 1)
         sinks = _check_int("sinks", sinks, 0)
         start = _check_int("query_start", start, 0)
     scale = float(scale)
@@ -166,9 +181,9 @@ def _attend(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor
             if table.dtype not in (torch.bfloat16, torch.float32):
                 raise ValueError(f"table must be bfloat16 or float32, got {table.dtype}")
             _register_buckets(buckets, max_distance)
-            if getattr(table, "main_grad", None) is not None and table.requires_grad and torch.is_grad_enabled():
-                table = _ToMainGrad.apply(table)
-        return _operator(q.device.index)(q, k, v, table, scale, window, sinks, start, max_distance)
+        out = _operator(q.device.index)(q, k, v, _trained(table), scale, window, sinks, start, max_distance)
+        if out is not None:
+            return out
     return _expression(q, k, v, table, max_distance, scale, window, sinks, start)
 
 
@@ -189,7 +204,7 @@ def relative_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, scal
     given.  Entries of ``-inf`` mask their bucket."""
     if table is None:
         raise TypeError("table must be a tensor")
-    return _attend(q, k, v, table, max_distance, scale, window, sinks, query_start)
+    return _attend(q, k, v, table, max_distance, scale, _INT_MAX if window is None else window, sinks, query_start)
 
 
 def _expression(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor:
