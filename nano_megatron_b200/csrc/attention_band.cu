@@ -507,7 +507,7 @@ template <int D, bool kExact>
 __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_constant__ BandFwdParams p) {
   using L = BandFwdSmem<D>;
   constexpr int NS = L::kSlabs, ST = L::kStages;
-  constexpr bool kOwn = D == 64;  // P has its own columns
+  constexpr bool kOwn = D == 64 && !kExact;  // P has its own columns
   constexpr int kIssuers = kOwn ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
   uint64_t* p_full = q_full + 6;
   uint64_t* o_full = q_full + 8;
   uint64_t* o_empty = q_full + 10;
-  uint64_t* s_read = q_full + 12;        // only with P's own columns
+  uint64_t* s_read = q_full + 12;        // only with P's own columns, as the next
   uint64_t* pv_done = q_full + 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -651,21 +651,18 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         // O += P V of tile u, whose V and P are there
         auto pv = [&](int i, int u, bool last) {
           const int t = t0 + i;
-          const uint32_t b_low = desc_mn(ring + ((base + 2 * u + 1) % ST) * L::kTile);
-#pragma unroll
-          for (int part = 0; part < (kExact ? 2 : 1); ++part) {  // the weights, then what was cut off of them
-            if (part == 1 && !band_wait(p_bar(i).bar, p_bar(i).parity, abort_flag, a.status, 77)) return false;
-            tc_fence_after();
-            if (one) {
-              mma_apply<8, kOwn ? 8 : 4, 64>(tmem + 256 + t * D, tmem + (kOwn ? 384 + t * 64 : t * 128), b_low, idesc_o, first_pv[i]);
-              if (kOwn || kExact) tc_commit(&pv_done[t]);
-              if (last && (!kExact || part == 1)) tc_commit(&o_full[t]);
-            }
-            ++n_p[i];
-            first_pv[i] = false;
+          tc_fence_after();
+          if (one) {
+            const uint32_t b_low = desc_mn(ring + ((base + 2 * u + 1) % ST) * L::kTile);
+            const uint32_t to = tmem + 256 + t * D, p_at = tmem + (kOwn ? 384 + t * 64 : t * 128);
+            mma_apply<8, kOwn ? 8 : 4, 64>(to, p_at, b_low, idesc_o, first_pv[i]);
+            if (kExact) mma_apply<8, 4, 64>(to, p_at + 32, b_low, idesc_o, false);
+            if (kOwn) tc_commit(&pv_done[t]);
+            if (last) tc_commit(&o_full[t]);
           }
+          ++n_p[i];
+          first_pv[i] = false;
           pending[i] = false;
-          return true;
         };
         auto o_free = [&](int i) {  // the accumulator, for the first product of an item
           return !first_pv[i] || n_item[i] == 0 || band_wait(&o_empty[t0 + i], (n_item[i] - 1) & 1, abort_flag, a.status, 64);
@@ -700,7 +697,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
             if (ok) release(base + 2 * u);
             if (ok && was) {
               ok = o_free(0) && band_wait_all(abort_flag, a.status, 63, v_bar(u - 1), p_bar(0));
-              ok = ok && pv(0, u - 1, left[0] == 0 && !use);
+              if (ok) pv(0, u - 1, left[0] == 0 && !use);
             }
             if (ok && u > 0) {  // V of a tile that only the other slot works on: passed on once it is there, not before
               if (!was) ok = band_wait(v_bar(u - 1).bar, v_bar(u - 1).parity, abort_flag, a.status, 76);
@@ -716,7 +713,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
                 ok = o_free(i) && (k_there && v_there ? band_wait(p_bar(i).bar, p_bar(i).parity, abort_flag, a.status, 65)
                                                       : band_wait_all(abort_flag, a.status, 65, k_bar(u), v_bar(u - 1), p_bar(i)));
                 k_there = v_there = true;
-                ok = ok && pv(i, u - 1, left[i] == 0);
+                if (ok) pv(i, u - 1, left[i] == 0);
               }
               if (ok && use) {
                 ok = (k_there || band_wait(k_bar(u).bar, k_bar(u).parity, abort_flag, a.status, 66)) && scores(i, u);
@@ -738,7 +735,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
           if (ok && pending[i]) {
             ok = o_free(i) && band_wait_all(abort_flag, a.status, 65, v_bar(n - 1), p_bar(i));
             v_there = true;
-            ok = ok && pv(i, n - 1, true);
+            if (ok) pv(i, n - 1, true);
           }
         }
         if (ok && n > 0) {
@@ -761,7 +758,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
     const float sl2 = a.scale * kBandLog2e;
     float* lut = luts + t * entries;
     float* xch = reinterpret_cast<float*>(smem + L::kXch) + t * 256 + r;
-    int n_s = 0, n_pv = 0, n_item = 0, parity = 0;
+    int n_s = 0, n_item = 0, parity = 0;
     bool ok = true;
     // the other thread's value of this row
     auto other = [&](float mine) {
@@ -855,7 +852,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         const float alpha = m_new == m ? 1.f : ex2(m - m_new);  // m == -inf: 0
         const float shift = add - (m_new == -INFINITY ? 0.f : m_new);
         // The product of the tile before is done: with shared columns the scores came after it.
-        if (kOwn && n_pv > 0) NMB_BAND_WAIT(&pv_done[t], (n_pv - 1) & 1, 73);
+        if (kOwn && n_s > 1) NMB_BAND_WAIT(&pv_done[t], n_s & 1, 73);
         if (u > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
           tc_fence_after();
 #pragma unroll 1
@@ -870,13 +867,6 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         }
         const uint64_t mul_2 = pack2(mul, mul), shift_2 = pack2(shift, shift);
         uint64_t sum = pack2(0.f, 0.f);
-        auto pass_on = [&]() {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
-          ++n_pv;
-        };
         if constexpr (!kExact) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -909,13 +899,13 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
             }
             tmem_st_32x16(t_p + c * 16, pk);
           }
-          pass_on();
-          NMB_BAND_WAIT(&pv_done[t], (n_pv - 1) & 1, 78);
-          tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < 2; ++c) tmem_st_32x16(t_p + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(s[c]));
+          for (int c = 0; c < 2; ++c) tmem_st_32x16(t_p + 32 + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(s[c]));
         }
-        pass_on();
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
         float sum0, sum1;
         unpack2(sum, sum0, sum1);
         l = l * alpha + (sum0 + sum1);
@@ -1007,11 +997,12 @@ static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStr
   return make_tmap_bf16(m, ptr, 4, dims, strides, box);
 }
 
-// With kExact the weights go into O to twice bf16's digits, the head and what it cut off in two products one after the other.
+// With kExact the weights go into O to twice bf16's digits: the head and what it cut off lie in the columns that the scores were
+// in, and take a product each.
 // A bias table's gradient is a sum over dS in which O's error does not cancel: with bf16 weights it was 2.2 times as far from
 // the exact one as its own rounding at 22 keys, 1.4 times at most above 512 keys, where the errors average out; with both it is
 // no further at any.  So training with a table pays for the second product up to kExactKeys keys a row (8 x 512 rows, 16
-// heads, D = 64, window 128: 20 -> 27 us) and nothing else does.  A variant of its own: the test inside the loop cost the
+// heads, D = 64, window 128: 20 -> 24 us) and nothing else does.  A variant of its own: the test inside the loop cost the
 // others 10 percent through registers.
 constexpr int kExactKeys = 512;
 template <int D>
