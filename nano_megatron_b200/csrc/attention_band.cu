@@ -998,20 +998,21 @@ static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStr
 }
 
 // With kExact the weights go into O to twice bf16's digits: the head and what it cut off lie in the columns that the scores were
-// in, and take a product each.
-// A bias table's gradient is a sum over dS in which O's error does not cancel: with bf16 weights it was 2.2 times as far from
-// the exact one as its own rounding at 22 keys, 1.4 times at most above 512 keys, where the errors average out; with both it is
-// no further at any.  So training with a table pays for the second product up to kExactKeys keys a row (8 x 512 rows, 16
-// heads, D = 64, window 128: 20 -> 24 us) and nothing else does.  A variant of its own: the test inside the loop cost the
-// others 10 percent through registers.
-constexpr int kExactKeys = 512;
+// in, and take a product each.  D comes from O, and a bias table's gradient is a sum over dS in which D's error does not
+// cancel: with bf16 weights it was 2.2 times as far from the exact one as its own rounding at 22 keys, 1.4 times at most above
+// 512 keys, where the errors average out; with both parts it is no further at any.  dQ and dK, which also see dS rounded to
+// bf16, were 1.5 times as far as their own rounding at 2 keys and 1.46 at 64, and are 1.42 so.  So training pays for the
+// second product where rows see few keys (8 x 512 rows, 16 heads, D = 64, window 128, bias: 20 -> 24 us), and nothing else
+// does.  A variant of its own: the test inside the loop cost the others 10 percent through registers.
+static bool exact_weights(const BandArgs& a) {
+  const long long keys = std::min<long long>(a.Skv, static_cast<long long>(a.window) + a.sinks);
+  return a.rest_rows > 0 && keys <= (a.table != nullptr ? 512 : 64);
+}
 template <int D>
 static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
   const BandArgs& a = p.a;
   const int lut = a.table == nullptr ? 0 : lut_bytes(p.t_last, 2);
-  const bool exact = a.table != nullptr && a.rest_rows > 0 &&
-                     std::min<long long>(a.Skv, static_cast<long long>(a.window) + a.sinks) <= kExactKeys;
-  return launch_pdl(exact ? band_fwd_kernel<D, true> : band_fwd_kernel<D, false>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
+  return launch_pdl(exact_weights(a) ? band_fwd_kernel<D, true> : band_fwd_kernel<D, false>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
 }
 
 // --------------------------------------------------------------- backward --

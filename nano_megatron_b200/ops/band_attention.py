@@ -18,7 +18,9 @@ a data-parallel wrapper), else through autograd.
 bf16 CUDA tensors with a head_dim of 64, 96 or 128 go to the kernels; everything else (CPU, fp32, other
 head sizes) to the plain expression at the end of this file, in fp32 or wider.  The kernels multiply whole
 tiles of 128 keys, with zero weights where a key is masked: as in the plain expression, keys and values have
-to be finite in masked places too.
+to be finite in masked places too.  Where rows see few keys, a call that will be differentiated carries the
+weights to twice bf16's digits, for the gradients' sake: its output may differ from that of the same call without
+gradients by the roundings of the weights.  Results do not depend on timing: the same call gives the same bits.
 """
 from __future__ import annotations
 

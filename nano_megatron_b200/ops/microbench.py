@@ -2,6 +2,7 @@
 
     python -m nano_megatron_b200.ops.microbench gemm --m 4096 --n 4096 --k 1024
     python -m nano_megatron_b200.ops.microbench attn --batch 2 --seq 2048 --heads 16 --dim 64
+    python -m nano_megatron_b200.ops.microbench band --seq 8192 --heads 16 --dim 128
     python -m nano_megatron_b200.ops.microbench norm | ce | adamw | all
 
 Every kernel is timed with CUDA events after warm-up; between timed launches a

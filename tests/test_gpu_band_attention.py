@@ -374,3 +374,19 @@ def test_gradient_of_the_bias_over_few_keys(sq, hq, hkv, d, window, buckets, max
     bound = torch.zeros_like(values["dtable"]).index_add_(1, at.flatten(), terms.sum(0).flatten(1))
     assert ((got.double() - values["dtable"]).abs() <= bound + 1e-30).all(), \
         f"{((got.double() - values['dtable']).abs() / (bound + 1e-30)).max().item():.2f} times what is allowed"
+
+
+@pytest.mark.parametrize("sq,skv,hq,hkv,d,window,sinks,buckets", [
+    (28, 50, 4, 4, 64, 2, 0, 0), (300, 300, 4, 2, 96, 40, 24, 0), (64, 64, 2, 1, 128, 1000, 0, 0), (257, 257, 2, 2, 64, 100, 3, 12)])
+def test_output_over_few_keys_in_training(sq, skv, hq, hkv, d, window, sinks, buckets):
+    """The weights have twice bf16's digits then, for the sake of the gradients: 2^-17 of sum_j P_j |V_j|, as much for what is
+    held in fp32, and the result's own rounding are all that the output may be off."""
+    q, k, v, table, _ = _tensors(2, sq, skv, hq, hkv, d, buckets)
+    out = _call(q, k, v, table, d ** -0.5, 60, window=window, sinks=sinks, query_start=skv - sq)
+    assert out.requires_grad
+    values, bounds, _ = oracle(q, k, v, torch.zeros_like(q), d ** -0.5, window=window, sinks=sinks, start=skv - sq, table=table,
+                               max_distance=60)
+    half = torch.finfo(torch.bfloat16).eps / 2
+    size = (bounds["out"] - half * values["out"].abs()) / (half + 2.0 ** -13)  # sum_j P_j |V_j|: the oracle's bound without its parts
+    bound = half * values["out"].abs() + (1 + half) * 2.0 ** -16 * size
+    assert ((out.double() - values["out"]).abs() <= bound).all()
