@@ -2114,7 +2114,7 @@ __global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant_
 static void plan_pieces(BandBwdParams& p) {
   const BandArgs& a = p.a;
   const int sms = sm_count(), n_hb = a.Hkv * a.B, piece_cost = 2 + a.d / 32;
-  constexpr int kMaxRounds = 16;  // those after them are alike, and cutting gains nothing where there are as many
+  constexpr int kMaxRounds = 16;  // looked at one by one; cutting gains nothing where there are more
   int longest = 1, longest_sink = 1;
   for (int t = 0; t < p.n_kt; ++t) {
     int& most = t < p.sink_tiles ? longest_sink : longest;
@@ -2122,28 +2122,33 @@ static void plan_pieces(BandBwdParams& p) {
   }
   const int others = p.n_kt - p.sink_tiles;
   p.pieces = p.sink_pieces = 1;
-  int best = INT_MAX;
+  long long best = LLONG_MAX;
+  const long long looked_at = static_cast<long long>(kMaxRounds) * sms;
   for (int c : {1, 2, 3, 4, 6, 8, 12, 16}) {
-    if (c > 1 && (c > longest || static_cast<long long>(others) * c * n_hb > static_cast<long long>(kMaxRounds) * sms)) break;
+    if (c > 1 && (c > longest || static_cast<long long>(others) * c * n_hb > looked_at)) break;
     const int piece = (longest + c - 1) / c;
     const int even = p.sink_tiles == 0 ? 1 : std::min(64, (longest_sink + std::max(piece, 4) - 1) / std::max(piece, 4));
     for (int cs : {1, even}) {
       const long long sink_items = static_cast<long long>(p.sink_tiles) * cs * n_hb;
       const long long items = sink_items + static_cast<long long>(others) * c * n_hb;
+      if (cs > 1 && sink_items > looked_at) break;
+      const int of_sink = (longest_sink + cs - 1) / cs + (cs > 1 ? piece_cost : 2), of_other = piece + (c > 1 ? piece_cost : 2);
       const int rounds = static_cast<int>(std::min<long long>((items + sms - 1) / sms, kMaxRounds));
-      int cost = 0;
+      long long cost = 0;
       for (int part = 0; part < 5; ++part) {
         const int sm = part * (sms - 1) / 4;
         int load = 0;
         for (int round = 0; round < rounds; ++round) {
           const long long i = static_cast<long long>(round) * sms + ((round & 1) ? sms - 1 - sm : sm);
           if (i >= items) break;
-          if (i < sink_items) load += (longest_sink + cs - 1) / cs + (cs > 1 ? piece_cost : 2);
+          if (i < sink_items) load += of_sink;
           else if (const int steps = dkv_steps(a, other_tile(p, static_cast<int>((i - sink_items) / n_hb / c))))
             load += (steps + c - 1) / c + (c > 1 ? piece_cost : 2);
         }
-        cost = std::max(cost, load);
+        cost = std::max<long long>(cost, load);
       }
+      const long long sinks_after = std::max<long long>(0, sink_items - looked_at), after = std::max<long long>(0, items - looked_at);
+      cost += (sinks_after * of_sink + (after - sinks_after) * of_other) / sms;
       if (c > 1 || (cs > 1 && p.sink_tiles > 0)) cost += 2;
       if (cost < best) {
         best = cost;

@@ -122,7 +122,7 @@ def _check_int(name: str, value, low: int) -> int:
     if isinstance(value, bool) or not isinstance(value, int):
         raise TypeError(f"{name} must be an int, got {type(value).__name__}")
     if not low <= value <= _INT_MAX:
-        raise ValueError(f"{name} must be at least {low}, got {value}")
+        raise ValueError(f"{name} must be at least {low} and below 2 ** 31, got {value}")
     return value
 
 
@@ -164,10 +164,9 @@ def _attend(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor
         raise ValueError(f"q, k, v must share a floating type; got {q.dtype}, {k.dtype}, {v.dtype}")
     if not q.device == k.device == v.device:
         raise ValueError(f"q, k, v must be on one device; got {q.device}, {k.device}, {v.device}")
-    if type(window) is not int or type(sinks) is not int or type(start) is not int or window < 1 or sinks < 0 or start < 0:
-        window = _check_int("window", window, 1)
-        sinks = _check_int("sinks", sinks, 0)
-        start = _check_int("query_start", start, 0)
+    window = _check_int("window", window, 1)
+    sinks = _check_int("sinks", sinks, 0)
+    start = _check_int("query_start", start, 0)
     scale = float(scale)
     buckets = None
     if table is not None:

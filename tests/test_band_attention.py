@@ -94,7 +94,7 @@ def _good():
 @pytest.mark.parametrize("change,error", [
     (dict(window=0), ValueError), (dict(window=-1), ValueError), (dict(window=2.0), TypeError), (dict(window=True), TypeError),
     (dict(window=None), TypeError), (dict(sinks=-1), ValueError), (dict(sinks=1.5), TypeError), (dict(query_start=-1), ValueError),
-    (dict(query_start=2 ** 30), ValueError), (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError),
+    (dict(query_start=2 ** 30), ValueError), (dict(window=2 ** 40), ValueError), (dict(sinks=2 ** 31), ValueError), (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError),
     (dict(scale=float("nan")), ValueError), (dict(scale=float("inf")), ValueError)])
 def test_refused_numbers(change, error):
     q, k, v, _ = _good()

@@ -390,3 +390,44 @@ def test_output_over_few_keys_in_training(sq, skv, hq, hkv, d, window, sinks, bu
     size = (bounds["out"] - half * values["out"].abs()) / (half + 2.0 ** -13)  # sum_j P_j |V_j|: the oracle's bound without its parts
     bound = half * values["out"].abs() + (1 + half) * 2.0 ** -16 * size
     assert ((out.double() - values["out"]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("sq,h,window,sinks", [(65536, 16, 64, 65536), (65536, 128, 64, 128), (16384, 64, 1024, 16384), (8192, 2, 1024, 16)])
+def test_scratch_stays_small(sq, h, window, sinks):
+    """Key tiles are cut where SMs would be idle, not where there are enough of them: pieces of 128 x (dK, dV) in fp32."""
+    from nano_megatron_b200.ops import native
+
+    args = _Args(B=1, Hq=h, Hkv=h, Sq=sq, Skv=sq, d=128, window=window, sinks=sinks, scale=1.0)
+    floats = native.lib().nmb_band_bwd_scratch(ctypes.byref(args))
+    stats = h * (sq // 128) * 512
+    assert stats <= floats <= stats + 16 * 148 * 128 * 256
+    if h * sq // 128 >= 16 * 148:
+        assert floats == stats or sinks < sq, "more key tiles than 16 for each SM are not cut"
+
+
+def test_refusals_where_the_kernels_run():
+    from nano_megatron_b200.ops.band_attention import relative_bias_attention, window_attention
+
+    q, k, v, table, _ = _tensors(1, 70, 70, 4, 2, 64, 8)
+    window_attention(q, k, v, 0.125, window=9)  # the operator is there: what follows is looked at from C++ first
+    for kw, error in ((dict(window=0), ValueError), (dict(window=2.0), TypeError), (dict(window=True), TypeError),
+                      (dict(window=3, sinks=-1), ValueError), (dict(window=3, query_start=-1), ValueError),
+                      (dict(window=3, query_start=2 ** 30), ValueError), (dict(window=2 ** 40), ValueError)):
+        with pytest.raises(error):
+            window_attention(q, k, v, 0.125, **kw)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            window_attention(q, k, v, scale, window=3)
+    for bad in ((q[0], k, v), (q, k, v[:, :3]), (q[..., :32], k, v), (q[:, :, :3], k, v), (q.float(), k, v), (q, k.cpu(), v.cpu()),
+                (q.expand(2, -1, -1, -1), k, v), (q, k[:, :, :0], v[:, :, :0])):
+        with pytest.raises(ValueError):
+            window_attention(*bad, 0.125, window=2)
+    for bad in (table[:2], table[0], table[:, :1], table.cpu(), table.half(), torch.zeros(4, 129, device="cuda")):
+        with pytest.raises(ValueError):
+            relative_bias_attention(q, k, v, bad, 0.125)
+    for distance, error in ((4, ValueError), (2049, ValueError), (8.0, TypeError)):
+        with pytest.raises(error):
+            relative_bias_attention(q, k, v, table, 0.125, max_distance=distance)
+    for empty in (q[:0], q[:, :0]):
+        assert window_attention(empty, k[:empty.shape[0]], v[:empty.shape[0]], 0.125, window=3).shape == empty.shape
+    assert (window_attention(q, k[:, :0], v[:, :0], 0.125, window=3) == 0).all()
