@@ -124,7 +124,7 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
 // the whole warp by construction, which is where the instruction wants them (uniform registers).  With the loops inside a
 // branch of one lane every operand was moved there first and issuing, not the tensor core, set the pace (a step of two slots
 // at d = 128: 4160 clocks to issue 32 products that take 2048).
-__device__ __forceinline__ bool elect_one() {
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t e;
   asm volatile(
       "{\n\t"
@@ -133,7 +133,7 @@ __device__ __forceinline__ bool elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t"
       "}"
       : "=r"(e));
-  return e != 0;
+  return e;
 }
 // Shared-memory operands: the low word of a descriptor (address and the stride between slabs of an MN-major operand) moves
 // from product to product, the high word does not.
@@ -141,49 +141,65 @@ constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row
 __device__ __forceinline__ uint32_t desc_k(uint32_t smem) { return ((smem & 0x3ffff) >> 4) | (1u << 16); }
 __device__ __forceinline__ uint32_t desc_mn(uint32_t smem) { return ((smem & 0x3ffff) >> 4) | ((16384u >> 4) << 16); }
 
+// (`one`: see commit_one)
 template <bool kAccumulate>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t one) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p;\n\t"
+      ".reg .pred p, q;\n\t"
       ".reg .b64 a, b;\n\t"
       "mov.b64 a, {%1, %5};\n\t"
       "mov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
       "}" ::"r"(d),
-      "r"(a_low), "r"(b_low), "r"(idesc), "n"(kAccumulate ? 1 : 0), "n"(kDescHigh)
+      "r"(a_low), "r"(b_low), "r"(idesc), "n"(kAccumulate ? 1 : 0), "n"(kDescHigh), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate, uint32_t one) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p;\n\t"
+      ".reg .pred p, q;\n\t"
       ".reg .b64 b;\n\t"
       "mov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
       "}" ::"r"(d),
-      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(one)
+      : "memory");
+}
+// A commit by the lanes with `one`, as a predicate instead of a branch around it.  Products and commits without branches, for
+// the whole warp in one stream of instructions, took 1 to 3 percent off the forward kernel at D > 64 (one issuer, two slots) and
+// added 1 to 2 percent elsewhere.
+__device__ __forceinline__ void commit_one(uint64_t* bar, uint32_t one) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+      "}" ::"r"(smem_u32(bar)), "r"(one)
       : "memory");
 }
 // D[128 x 128] = A B^T over a depth of D, both K-major; one lane
 template <int D>
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc) {
-  mma_ss<false>(d, a_low, b_low, idesc);
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t one = 1) {
+  mma_ss<false>(d, a_low, b_low, idesc, one);
 #pragma unroll
   for (int k = 1; k < D / 16; ++k) {
     const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-    mma_ss<true>(d, a_low + off, b_low + off, idesc);
+    mma_ss<true>(d, a_low + off, b_low + off, idesc, one);
   }
 }
 // D[128 x n] (+)= A B over a depth of 16 kSteps, A bf16 in tensor memory (kPer steps side by side, the next kStride columns
 // on), B MN-major; one lane
 template <int kSteps, int kPer, int kStride>
-__device__ __forceinline__ void mma_apply(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, bool first) {
-  mma_ts(d, a_tmem, b_low, idesc, first ? 0u : 1u);
+__device__ __forceinline__ void mma_apply(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, bool first,
+                                          uint32_t one = 1) {
+  mma_ts(d, a_tmem, b_low, idesc, first ? 0u : 1u, one);
 #pragma unroll
-  for (int k = 1; k < kSteps; ++k) mma_ts(d, a_tmem + (k / kPer) * kStride + (k % kPer) * 8, b_low + k * (2048 >> 4), idesc, 1u);
+  for (int k = 1; k < kSteps; ++k) mma_ts(d, a_tmem + (k / kPer) * kStride + (k % kPer) * 8, b_low + k * (2048 >> 4), idesc, 1u, one);
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -619,7 +635,9 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
       constexpr int kMine = 2 / kIssuers;  // slots of an issuer
       const uint32_t ring = smem_u32(smem + L::kRing);
       const int t0 = kOwn ? warp - kMmaWarp : 0;
-      const bool one = elect_one();
+      const uint32_t chosen = elect_one();
+      const bool branch = kOwn ? chosen != 0 : true;
+      const uint32_t one = kOwn ? 1 : chosen;
       uint32_t base = 0, n_s[kMine] = {}, n_p[kMine] = {}, n_item[kMine] = {};
       bool ok = true;
       for (int round = 0; ok; ++round) {
@@ -652,13 +670,13 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         auto pv = [&](int i, int u, bool last) {
           const int t = t0 + i;
           tc_fence_after();
-          if (one) {
+          if (branch) {
             const uint32_t b_low = desc_mn(ring + ((base + 2 * u + 1) % ST) * L::kTile);
             const uint32_t to = tmem + 256 + t * D, p_at = tmem + (kOwn ? 384 + t * 64 : t * 128);
-            mma_apply<8, kOwn ? 8 : 4, 64>(to, p_at, b_low, idesc_o, first_pv[i]);
-            if (kExact) mma_apply<8, 4, 64>(to, p_at + 32, b_low, idesc_o, false);
-            if (kOwn) tc_commit(&pv_done[t]);
-            if (last) tc_commit(&o_full[t]);
+            mma_apply<8, kOwn ? 8 : 4, 64>(to, p_at, b_low, idesc_o, first_pv[i], one);
+            if (kExact) mma_apply<8, 4, 64>(to, p_at + 32, b_low, idesc_o, false, one);
+            if (kOwn) commit_one(&pv_done[t], one);
+            if (last) commit_one(&o_full[t], one);
           }
           ++n_p[i];
           first_pv[i] = false;
@@ -675,16 +693,16 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
           ++n_s[i];
           tc_fence_after();
           const bool last = --left[i] == 0;
-          if (one) {
+          if (branch) {
             mma_scores<D>(tmem + t * 128, desc_k(smem_u32(smem + L::kQ + t * L::kTile)),
-                          desc_k(ring + ((base + 2 * u) % ST) * L::kTile), idesc_s);
-            tc_commit(&s_full[t]);
-            if (last) tc_commit(&q_empty[t]);
+                          desc_k(ring + ((base + 2 * u) % ST) * L::kTile), idesc_s, one);
+            commit_one(&s_full[t], one);
+            if (last) commit_one(&q_empty[t], one);
           }
           return true;
         };
         auto release = [&](uint32_t pos) {
-          if (one) tc_commit(&kv_empty[pos % ST]);
+          if (branch) commit_one(&kv_empty[pos % ST], one);
         };
         for (int u = 0; u < n && ok; ++u) {
           const int j = tile_at(w.all, u);
