@@ -441,7 +441,7 @@ __device__ __forceinline__ int item_of_round(int round) {
 
 // ---------------------------------------------------------------- forward --
 // A CTA works on two query tiles ("slots") at a time against the same key tiles: two heads of a group where the group is
-// even, else two neighbouring tiles of a head, else (few tiles in all) one.  While the softmax warps of one slot turn its
+// even, else two neighbouring tiles of a head, else (few tiles in all) one, or a piece of one's keys.  While the softmax warps of one slot turn its
 // scores into weights the tensor core works on the other's.  640 threads:
 //   warps 0-7, 8-15  softmax of slot 0, 1: two threads per query row, 64 keys each, that agree on the maximum through shared
 //                    memory.  One thread per row left two warps per scheduler, whose latencies nothing covered.
@@ -468,6 +468,9 @@ struct BandFwdParams {
   int s_pad;    // rows of the statistics: n_qt * 128
   int n_items;
   int t_last;   // first distance of the last bucket
+  int pieces;   // parts of a tile's keys, with pair == 0 only: sums and statistics of each go to `part`
+  float* part;  // per item: [128][D], then m [128] and l [128]
+  FastDiv by_pieces;
   FastDiv by_hb, by_heads, by_group;  // heads (or pairs of them) times batches; heads (or pairs); query heads of a key head
 };
 
@@ -486,16 +489,26 @@ struct BandFwdSmem {
   static constexpr int kLut = kXch + 4096;                                     // float [2][entries], then the map
 };
 
+template <int D>
+constexpr int kFwdPart = 128 * D + 256;  // floats
+
 struct FwdItem {
   int b, hk;
+  int slot;  // of a piece; -1: the whole
   int h[2], q0[2];
   KeyTiles t[2], all;
 };
 
+template <bool kSplit>
 __device__ __forceinline__ FwdItem fwd_item(const BandFwdParams& p, int item) {
   const BandArgs& a = p.a;
   FwdItem w;
-  int rest, h;
+  int rest, h, piece = 0;
+  w.slot = -1;
+  if (kSplit) {
+    w.slot = item;
+    item = p.by_pieces.quot(item, piece);
+  }
   const int tiles = p.pair == 1 ? (p.n_qt + 1) / 2 : p.n_qt;
   const int tile = tiles - 1 - p.by_hb.quot(item, rest);
   w.b = p.by_heads.quot(rest, h);
@@ -505,6 +518,14 @@ __device__ __forceinline__ FwdItem fwd_item(const BandFwdParams& p, int item) {
   w.q0[0] = (p.pair == 1 ? 2 * tile : tile) * 128;
   w.q0[1] = p.pair == 1 ? w.q0[0] + 128 : w.q0[0];
   w.t[0] = key_tiles(a, w.q0[0]);
+  if (kSplit) {  // the first piece has the sinks too
+    const int first = w.t[0].lo, n = w.t[0].hi - first + 1;
+    if (n > 0) {
+      w.t[0].lo = first + n * piece / p.pieces;
+      w.t[0].hi = first + n * (piece + 1) / p.pieces - 1;
+    }
+    if (piece > 0) w.t[0].sink = 0;
+  }
   if (p.pair == 0 || w.q0[1] >= a.Sq) {
     w.q0[1] = -1;
     w.t[1].sink = 0;
@@ -519,7 +540,7 @@ __device__ __forceinline__ FwdItem fwd_item(const BandFwdParams& p, int item) {
   return w;
 }
 
-template <int D, bool kExact>
+template <int D, bool kExact, bool kSplit>
 __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_constant__ BandFwdParams p) {
   using L = BandFwdSmem<D>;
   constexpr int NS = L::kSlabs, ST = L::kStages;
@@ -598,7 +619,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         const int item = item_of_round(round);
         if (round * static_cast<int>(gridDim.x) >= p.n_items) break;
         if (item >= p.n_items) continue;
-        const FwdItem w = fwd_item(p, item);
+        const FwdItem w = fwd_item<kSplit>(p, item);
         auto load = [&](const CUtensorMap* m, int j) {
           const int st = pos % ST, use = pos / ST;
           if (use > 0 && !band_wait(&kv_empty[st], (use - 1) & 1, abort_flag, a.status, 61)) return false;
@@ -644,7 +665,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         const int item = item_of_round(round);
         if (round * static_cast<int>(gridDim.x) >= p.n_items) break;
         if (item >= p.n_items) continue;
-        const FwdItem w = fwd_item(p, item);
+        const FwdItem w = fwd_item<kSplit>(p, item);
         const int n = w.all.count();
         KeyTiles mine[kMine];
         int left[kMine];
@@ -790,7 +811,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
       const int item = item_of_round(round);
       if (round * static_cast<int>(gridDim.x) >= p.n_items) break;
       if (item >= p.n_items) continue;
-      const FwdItem w = fwd_item(p, item);
+      const FwdItem w = fwd_item<kSplit>(p, item);
       const int q0 = t == 0 ? w.q0[0] : w.q0[1], h = t == 0 ? w.h[0] : w.h[1];
       const KeyTiles mine = t == 0 ? w.t[0] : w.t[1];
       if (q0 < 0) continue;
@@ -935,6 +956,33 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         ++n_item;
         tc_fence_after();
       }
+      if (kSplit) {
+        float* part = p.part + static_cast<long long>(w.slot) * kFwdPart<D>;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[16];
+          if (n > 0) {
+            tmem_ld_32x16(t_o + c * 16, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = 0;
+          }
+          float* at = part + r * D + half * (D / 2) + c * 16;
+          st_global_32(at, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]);
+          st_global_32(at + 8, o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]);
+        }
+        if (half == 0) {
+          part[128 * D + r] = m;
+          part[128 * D + 128 + r] = l;
+        }
+        if (n > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[t]);
+        }
+        continue;
+      }
       const float inv = l > 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* out = band_row(a.o, a.o_st, w.b, row, h) + half * (D / 2);
       uint8_t* tile = smem + L::kOut + 2 * t * L::kTile;
@@ -1007,6 +1055,44 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
   }
 }
 
+// What the pieces of a query tile come to: a warp per row, the pieces in order.  A piece that saw no key has m = -inf, l = 0.
+template <int D>
+__global__ void __launch_bounds__(256) band_join_kernel(const __grid_constant__ BandFwdParams p) {
+  pdl_enter();
+  const BandArgs& a = p.a;
+  const int lane = threadIdx.x & 31, at = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5), item = at >> 7, r = at & 127;
+  int rest, h;
+  const int row = (p.n_qt - 1 - p.by_hb.quot(item, rest)) * 128 + r, b = p.by_heads.quot(rest, h);
+  if (row >= a.Sq) return;
+  const float* part = p.part + static_cast<long long>(item) * p.pieces * kFwdPart<D>;
+  float top = -INFINITY;
+  for (int i = 0; i < p.pieces; ++i) top = fmaxf(top, part[static_cast<long long>(i) * kFwdPart<D> + 128 * D + r]);
+  float sum = 0.f, o[D / 32] = {};
+  if (top != -INFINITY) {
+    for (int i = 0; i < p.pieces; ++i) {
+      const float* one = part + static_cast<long long>(i) * kFwdPart<D>;
+      const float w = ex2(one[128 * D + r] - top);
+      sum = fmaf(w, one[128 * D + 128 + r], sum);
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) o[k] = fmaf(w, one[r * D + k * 32 + lane], o[k]);
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  __nv_bfloat16* out = band_row(a.o, a.o_st, b, row, h);
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) {
+    const float x = o[k] * inv;
+    const __nv_bfloat16 y = __float2bfloat16(x);
+    out[k * 32 + lane] = y;
+    if (row < a.rest_rows) rest_row(a, b, row, h, D)[k * 32 + lane] = __float2bfloat16(x - __bfloat162float(y));
+  }
+  if (lane == 0 && a.m != nullptr) {
+    const long long stat = (static_cast<long long>(b) * a.Hq + h) * a.Sq + row;
+    a.m[stat] = sum > 0.f ? top : INFINITY;
+    a.l[stat] = sum > 0.f ? log2f(sum) : 0.f;
+  }
+}
+
 static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStride& t, int d, int S, int H, int B) {
   const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(S), static_cast<uint64_t>(H), static_cast<uint64_t>(B)};
   const uint64_t strides[3] = {static_cast<uint64_t>(t.s) * 2, static_cast<uint64_t>(t.h) * 2,
@@ -1030,7 +1116,25 @@ template <int D>
 static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
   const BandArgs& a = p.a;
   const int lut = a.table == nullptr ? 0 : lut_bytes(p.t_last, 2);
-  return launch_pdl(exact_weights(a) ? band_fwd_kernel<D, true> : band_fwd_kernel<D, false>, dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
+  const bool exact = exact_weights(a);
+  return launch_pdl(p.pieces > 1 ? (exact ? band_fwd_kernel<D, true, true> : band_fwd_kernel<D, false, true>)
+                                 : (exact ? band_fwd_kernel<D, true, false> : band_fwd_kernel<D, false, false>), dim3(std::min(p.n_items, sm_count())), dim3(kBandThreads), BandFwdSmem<D>::kLut + lut, s, p);
+}
+template <int D>
+static cudaError_t launch_band_join(const BandFwdParams& p, cudaStream_t s) {
+  return launch_pdl(band_join_kernel<D>, dim3(static_cast<unsigned>(p.n_items / p.pieces * 16)), dim3(256), 0, s, p);
+}
+// Into how many pieces the keys of a query tile are cut where there are not half as many tiles as SMs, four key tiles to a piece
+// at least: one row over 8192 keys, 16 heads of 128: 115 -> 25 us; over 1024 keys 18 -> 15 us.  (As a variant of its own: the
+// pieces cost the others 2 to 5 percent.)
+constexpr int kSplitKeyTiles = 8;
+static int fwd_pieces(const BandArgs& a) {
+  const long long tiles = static_cast<long long>((a.Sq + 127) / 128) * a.Hq * a.B;
+  if (tiles * 2 > sm_count()) return 1;
+  const long long seen = std::min<long long>(std::min<long long>(a.Skv, static_cast<long long>(a.q_pos0) + a.Sq), a.window + 127ll);
+  const int n = static_cast<int>((seen + 127) / 128);
+  if (n < kSplitKeyTiles) return 1;
+  return std::min(static_cast<int>(sm_count() / tiles), (n + 3) / 4);
 }
 
 // --------------------------------------------------------------- backward --
@@ -2274,12 +2378,18 @@ extern "C" int nmb_band_configure() {
       e = cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   };
   const int lut = lut_bytes(kMaxDistance, 2);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, false>), BandFwdSmem<64>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, true>), BandFwdSmem<64>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, false>), BandFwdSmem<96>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, true>), BandFwdSmem<96>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, false>), BandFwdSmem<128>::kLut + lut);
-  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, true>), BandFwdSmem<128>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, false, false>), BandFwdSmem<64>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, false, true>), BandFwdSmem<64>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, true, false>), BandFwdSmem<64>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<64, true, true>), BandFwdSmem<64>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, false, false>), BandFwdSmem<96>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, false, true>), BandFwdSmem<96>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, true, false>), BandFwdSmem<96>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<96, true, true>), BandFwdSmem<96>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, false, false>), BandFwdSmem<128>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, false, true>), BandFwdSmem<128>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, true, false>), BandFwdSmem<128>::kLut + lut);
+  opt_in(reinterpret_cast<const void*>(band_fwd_kernel<128, true, true>), BandFwdSmem<128>::kLut + lut);
   const int lut1 = lut_bytes(kMaxDistance, 1);
   opt_in(reinterpret_cast<const void*>(band_bwd_dq_kernel<64>), BandDqSmem<64>::kLut + lut1 + BandDqSmem<64>::kBins);
   opt_in(reinterpret_cast<const void*>(band_bwd_dq_kernel<96>), BandDqSmem<96>::kLut + lut1 + BandDqSmem<96>::kBins);
@@ -2290,8 +2400,17 @@ extern "C" int nmb_band_configure() {
   return e == cudaSuccess ? 0 : 300 + e;
 }
 
-extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
+extern "C" long long nmb_band_fwd_scratch(const BandArgs* a) {
+  if (band_check(a)) return 0;
+  const int pieces = fwd_pieces(*a);
+  return pieces == 1 ? 0 : static_cast<long long>((a->Sq + 127) / 128) * a->Hq * a->B * pieces * (128 * a->d + 256);
+}
+
+extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) { return nmb_band_fwd_split(a, nullptr, stream); }
+
+extern "C" int nmb_band_fwd_split(const BandArgs* a, float* scratch, void* stream) {
   if (int bad = band_check(a)) return bad;
+  if (reinterpret_cast<uintptr_t>(scratch) % 32 != 0) return kBadArgument;
   (void)cudaGetLastError();
   BandFwdParams p;
   p.a = *a;
@@ -2309,7 +2428,10 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   const long long tiles = static_cast<long long>(p.n_qt) * a->Hq * a->B;
   // one tile an item while every tile can have an SM of its own
   p.pair = tiles <= sm_count() ? 0 : (a->Hq / a->Hkv) % 2 == 0 ? 2 : 1;
-  const long long items = p.pair == 0 ? tiles : p.pair == 2 ? tiles / 2 : static_cast<long long>((p.n_qt + 1) / 2) * a->Hq * a->B;
+  p.pieces = scratch == nullptr ? 1 : fwd_pieces(*a);
+  p.part = scratch;
+  p.by_pieces = FastDiv(p.pieces);
+  const long long items = p.pair == 0 ? tiles * p.pieces : p.pair == 2 ? tiles / 2 : static_cast<long long>((p.n_qt + 1) / 2) * a->Hq * a->B;
   if (items > (1 << 30)) return kTooLarge;
   p.n_items = static_cast<int>(items);
   const int heads = p.pair == 2 ? a->Hq / 2 : a->Hq;
@@ -2317,8 +2439,12 @@ extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) {
   p.by_heads = FastDiv(heads);
   p.by_group = FastDiv(a->Hq / a->Hkv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->d == 64 ? launch_band_fwd<64>(p, s) : a->d == 96 ? launch_band_fwd<96>(p, s) : launch_band_fwd<128>(p, s);
+  cudaError_t e = a->d == 64 ? launch_band_fwd<64>(p, s) : a->d == 96 ? launch_band_fwd<96>(p, s) : launch_band_fwd<128>(p, s);
   if (e == cudaSuccess) ++g_band_launches;
+  if (e == cudaSuccess && p.pieces > 1) {
+    e = a->d == 64 ? launch_band_join<64>(p, s) : a->d == 96 ? launch_band_join<96>(p, s) : launch_band_join<128>(p, s);
+    if (e == cudaSuccess) ++g_band_launches;
+  }
   return e == cudaSuccess ? 0 : 400 + e;
 }
 

@@ -46,6 +46,10 @@ int nmb_band_args_size();
 // Floats of `scratch` that the backward pass of these arguments needs.
 long long nmb_band_bwd_scratch(const nmb::BandArgs* a);
 int nmb_band_fwd(const nmb::BandArgs* a, void* stream);
+// The same with the keys of a query tile cut into pieces where few tiles see many keys: floats of `scratch` that it takes then
+// (0: not cut), and the call, which does without where `scratch` is null.
+long long nmb_band_fwd_scratch(const nmb::BandArgs* a);
+int nmb_band_fwd_split(const nmb::BandArgs* a, float* scratch, void* stream);
 int nmb_band_bwd(const nmb::BandArgs* a, void* stream);
 // The two steps of the backward pass for a caller that makes `scratch` in between.
 int nmb_band_bwd_plan(const nmb::BandArgs* a, nmb::BandPlan* plan);

@@ -132,8 +132,10 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
       stats = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
     }
     const nmb::BandArgs a = arguments(q, k, v, table, out, rest, stats, scale, window, sinks, start, max_distance);
-    const int rc = nmb_band_fwd(&a, current_stream(q));
-    TORCH_CHECK(rc == 0, "nmb_band_fwd: launcher returned ", rc);
+    Tensor scratch;
+    if (const long long floats = nmb_band_fwd_scratch(&a)) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+    const int rc = nmb_band_fwd_split(&a, scratch.defined() ? scratch.data_ptr<float>() : nullptr, current_stream(q));
+    TORCH_CHECK(rc == 0, "nmb_band_fwd_split: launcher returned ", rc);
     if (train) {
       ctx->save_for_backward({q, k, v, table, out, rest, stats});
       ctx->saved_data["numbers"] =  // all of them exact in a double

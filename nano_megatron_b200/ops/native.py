@@ -99,6 +99,7 @@ def lib() -> ctypes.CDLL:
                     )
                 _lib = ctypes.CDLL(str(_LIB_PATH))
                 _lib.nmb_band_bwd_scratch.restype = ctypes.c_longlong
+                _lib.nmb_band_fwd_scratch.restype = ctypes.c_longlong
                 _lib.nmb_band_launches.restype = ctypes.c_longlong
                 pair = os.environ.get("NMB_GEMM_PAIR")
                 if pair is not None:

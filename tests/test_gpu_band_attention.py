@@ -431,3 +431,21 @@ def test_refusals_where_the_kernels_run():
     for empty in (q[:0], q[:, :0]):
         assert window_attention(empty, k[:empty.shape[0]], v[:empty.shape[0]], 0.125, window=3).shape == empty.shape
     assert (window_attention(q, k[:, :0], v[:, :0], 0.125, window=3) == 0).all()
+
+
+@pytest.mark.parametrize("b,sq,skv,hq,hkv,d,window,sinks,start,buckets", [
+    (1, 1, 8192, 4, 2, 64, 10 ** 6, 0, 8191, 0), (2, 3, 5000, 2, 1, 128, 3000, 130, 4990, 0), (1, 130, 2500, 2, 2, 96, None, 0, 2370, 32),
+    (1, 300, 4100, 3, 1, 64, 1500, 700, 3800, 16), (1, 1100, 1100, 1, 1, 128, None, 0, 0, 8), (1, 200, 3000, 2, 1, 96, 1100, 5, 2950, 0),
+    (1, 150, 2000, 2, 2, 64, 1200, 0, 3100, 0)])
+def test_few_rows_over_many_keys(b, sq, skv, hq, hkv, d, window, sinks, start, buckets):
+    """Cut into pieces of the keys, which are joined: also pieces that some rows, or all of them, see nothing of."""
+    from nano_megatron_b200.ops import native
+
+    args = _Args(B=b, Hq=hq, Hkv=hkv, Sq=sq, Skv=skv, d=d, q_pos0=start, window=min(window or 2 ** 30, 2 ** 30), sinks=min(sinks, skv), scale=1.0)
+    assert native.lib().nmb_band_fwd_scratch(ctypes.byref(args)) > 0
+    tensors = _tensors(b, sq, skv, hq, hkv, d, buckets)
+    _compare(*tensors, window=window, sinks=sinks, start=start)
+    q, k, v, table, _ = tensors
+    with torch.no_grad():
+        one, two = (_call(q, k, v, table, 0.1, 128, window=window, sinks=sinks, query_start=start) for _ in range(2))
+    assert torch.equal(one, two)
