@@ -449,3 +449,18 @@ def test_few_rows_over_many_keys(b, sq, skv, hq, hkv, d, window, sinks, start, b
     with torch.no_grad():
         one, two = (_call(q, k, v, table, 0.1, 128, window=window, sinks=sinks, query_start=start) for _ in range(2))
     assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+@pytest.mark.parametrize("sq,skv,hq,hkv,d,window,buckets,max_distance", [
+    (100, 3000, 4, 4, 128, None, 8, 60), (300, 2000, 8, 8, 96, None, 4, 20), (1024, 3000, 4, 2, 64, 1000, 24, 64)])
+def test_gradient_of_the_last_bucket(sq, skv, hq, hkv, d, window, buckets, max_distance, seed):
+    """The last bucket has nearly all keys of a row and the terms of its gradient cancel.  What is in the bf16 result besides its
+    own rounding is no larger than that: sqrt(2) of it in all, since the two are independent."""
+    start = skv - sq
+    q, k, v, table, dout = _tensors(1, sq, skv, hq, hkv, d, buckets, seed=seed)
+    out = _call(q, k, v, table, d ** -0.5, max_distance, window=window, query_start=start)
+    got = torch.autograd.grad(out, (q, k, v, table), dout)[3].double()
+    want = oracle(q, k, v, dout, d ** -0.5, window=window, start=start, table=table, max_distance=max_distance)[0]["dtable"]
+    rounding = (want.to(torch.bfloat16).double() - want).norm()
+    assert (got - want).norm() <= math.sqrt(2) * rounding, f"{((got - want).norm() / rounding).item():.2f} times its rounding"
