@@ -26,10 +26,10 @@ __device__ __forceinline__ float table_at(const BandArgs& p, int h, int b) {
   return p.table_fp32 ? static_cast<const float*>(p.table)[at]
                       : __bfloat162float(static_cast<const __nv_bfloat16*>(p.table)[at]);
 }
-// a table entry in the base-2 exponent domain
+// a table entry in the base-2 exponent domain; infinities and NaN stay
 __device__ __forceinline__ float bias_log2(float x) {
   const float y = x * kBandLog2e;
-  return isinf(x) ? x : fminf(fmaxf(y, -kBiasLimit), kBiasLimit);
+  return isfinite(x) ? fminf(fmaxf(y, -kBiasLimit), kBiasLimit) : x;
 }
 __device__ __forceinline__ __nv_bfloat16* rest_row(const BandArgs& a, int b, int s, int h, int d) {
   return a.o_rest + ((static_cast<long long>(b) * a.rest_rows + s) * a.Hq + h) * d;
@@ -206,9 +206,15 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Maxima that are NaN where one of the values is: a NaN among the scores of a row must not get lost.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // Two fp32 operations per instruction.
@@ -237,10 +243,13 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // by the polynomial of degree 4 with the smallest relative error on [-1/2, 1/2] (2.7e-6, found by exchange of extrema), 2^n
 // added to the exponent.  x below -126 gives 2^-126.  The exponential unit does 16 a clock and SM, a tile of 128 x 128 weights
 // 1024 clocks, as long as the tensor core takes for its products at d = 128; a part of the weights goes this way instead.
+// A NaN comes out as 2^-126, unless kNan asks for a NaN: then 2^n is a factor, since what is added to a NaN's bits can make
+// a number of it.  (Needed only where nothing else of the row's result shows the NaN.)
+template <bool kNan>
 __device__ __forceinline__ void exp2_pair_fma(uint64_t x2, float& y0, float& y1) {
   float x0, x1;
   unpack2(x2, x0, x1);
-  const uint64_t x = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t x = kNan ? pack2(max2(x0, -126.f), max2(x1, -126.f)) : pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
   const uint64_t t = add2(x, pack2(12582912.f, 12582912.f));
   const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
   const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
@@ -250,16 +259,22 @@ __device__ __forceinline__ void exp2_pair_fma(uint64_t x2, float& y0, float& y1)
   q = fma2(q, f, pack2(0.9999992847442627f, 0.9999992847442627f));
   float t0, t1, q0, q1;
   unpack2(t, t0, t1);
+  if (kNan) {
+    const uint64_t factor = pack2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
+                                  __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
+    unpack2(mul2(q, factor), y0, y1);
+    return;
+  }
   unpack2(q, q0, q1);
   y0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
   y1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
 }
 // One pair in this many takes that way.
 constexpr int kFmaPairs = 4;
-template <bool kMix>
+template <bool kMix, bool kNan = false>
 __device__ __forceinline__ void exp2_pair(int pair, uint64_t x2, float& y0, float& y1) {
   if (kMix && (pair % kFmaPairs) == kFmaPairs - 1) {
-    exp2_pair_fma(x2, y0, y1);
+    exp2_pair_fma<kNan>(x2, y0, y1);
   } else {
     float x0, x1;
     unpack2(x2, x0, x1);
@@ -880,14 +895,15 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
               m0 = max3(m0, __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
               m1 = max3(m1, __uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3]));
             }
-            mx[c] = max3(fmaxf(m0, m1), __uint_as_float(s[c][30]), __uint_as_float(s[c][31]));
+            mx[c] = max3(max2(m0, m1), __uint_as_float(s[c][30]), __uint_as_float(s[c][31]));
           }
         }
-        float top = fmaf(fmaxf(mx[0], mx[1]), mul, add);
-        top = fmaxf(top, other(top));
+        float top = fmaf(max2(mx[0], mx[1]), mul, add);
+        top = max2(top, other(top));
         // The maximum that weights are relative to moves only when it grew by more than 2^8: most tiles need no pass over O,
-        // and the division by the sum at the end makes the result exact.
-        const float m_new = top > m + 8.f ? top : m;
+        // and the division by the sum at the end makes the result exact.  A row with a score of NaN or +inf is NaN from here
+        // on: not all of its weights would be (a polynomial makes a quarter of them, which knows no NaN), but m is.
+        const float m_new = !(top < INFINITY) ? NAN : top > m + 8.f ? top : m;
         const float alpha = m_new == m ? 1.f : ex2(m - m_new);  // m == -inf: 0
         const float shift = add - (m_new == -INFINITY ? 0.f : m_new);
         // The product of the tile before is done: with shared columns the scores came after it.
@@ -947,7 +963,8 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         if (lane == 0) mbar_arrive(&p_full[t]);
         float sum0, sum1;
         unpack2(sum, sum0, sum1);
-        l = l * alpha + (sum0 + sum1);
+        // nothing but scores of -inf so far: the polynomial's 2^-126 for them are no weights
+        l = l * alpha + (m_new == -INFINITY ? 0.f : sum0 + sum1);
         m = m_new;
       }
       if (n > 0) {
@@ -983,7 +1000,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
         }
         continue;
       }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays
       __nv_bfloat16* out = band_row(a.o, a.o_st, w.b, row, h) + half * (D / 2);
       uint8_t* tile = smem + L::kOut + 2 * t * L::kTile;
       const bool some_rest = q0 < a.rest_rows;
@@ -1037,8 +1054,8 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_fwd_kernel(const __grid_
       }
       if (half == 0 && row < a.Sq && a.m != nullptr) {
         const long long stat = (static_cast<long long>(w.b) * a.Hq + h) * a.Sq + row;
-        a.m[stat] = l > 0.f ? m : INFINITY;  // a row that sees nothing: 2^(x - m) is 0 in the backward pass
-        a.l[stat] = l > 0.f ? log2f(l) : 0.f;
+        a.m[stat] = l == 0.f ? INFINITY : m;  // a row that sees nothing: 2^(x - m) is 0 in the backward pass
+        a.l[stat] = l == 0.f ? 0.f : log2f(l);
       }
     }
     if (L::kStage) store_wait();
@@ -1066,7 +1083,7 @@ __global__ void __launch_bounds__(256) band_join_kernel(const __grid_constant__ 
   if (row >= a.Sq) return;
   const float* part = p.part + static_cast<long long>(item) * p.pieces * kFwdPart<D>;
   float top = -INFINITY;
-  for (int i = 0; i < p.pieces; ++i) top = fmaxf(top, part[static_cast<long long>(i) * kFwdPart<D> + 128 * D + r]);
+  for (int i = 0; i < p.pieces; ++i) top = max2(top, part[static_cast<long long>(i) * kFwdPart<D> + 128 * D + r]);
   float sum = 0.f, o[D / 32] = {};
   if (top != -INFINITY) {
     for (int i = 0; i < p.pieces; ++i) {
@@ -1077,7 +1094,7 @@ __global__ void __launch_bounds__(256) band_join_kernel(const __grid_constant__ 
       for (int k = 0; k < D / 32; ++k) o[k] = fmaf(w, one[r * D + k * 32 + lane], o[k]);
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   __nv_bfloat16* out = band_row(a.o, a.o_st, b, row, h);
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) {
@@ -1088,8 +1105,8 @@ __global__ void __launch_bounds__(256) band_join_kernel(const __grid_constant__ 
   }
   if (lane == 0 && a.m != nullptr) {
     const long long stat = (static_cast<long long>(b) * a.Hq + h) * a.Sq + row;
-    a.m[stat] = sum > 0.f ? top : INFINITY;
-    a.l[stat] = sum > 0.f ? log2f(sum) : 0.f;
+    a.m[stat] = sum == 0.f ? INFINITY : top;
+    a.l[stat] = sum == 0.f ? 0.f : log2f(sum);
   }
 }
 
@@ -1145,7 +1162,7 @@ static int fwd_pieces(const BandArgs& a) {
 //   c = (far bias - m) - l,  D,  m,  l        (rows behind the last: c = -inf, so that their weights are 0)
 constexpr int kStatBlock = 512;  // floats
 
-// 2^(s * mul + shift) of 32 scores in place
+// 2^(s * mul + shift) of 32 scores in place (a NaN may get lost: D is one then, and with it dS)
 template <bool kMix>
 __device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, uint64_t shift) {
 #pragma unroll
@@ -1156,7 +1173,7 @@ __device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, uint64_t
     s[2 * k + 1] = __float_as_uint(p1);
   }
 }
-// the same with a shift per column
+// the same with a shift per column, and NaN where a score or a shift is one: these weights also go into dV, without D
 template <bool kMix>
 __device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, const float* shift) {
 #pragma unroll
@@ -1165,7 +1182,7 @@ __device__ __forceinline__ void exps32(uint32_t (&s)[32], uint64_t mul, const fl
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float p0, p1;
-      exp2_pair<kMix>(k + i, fma2(pack2(__uint_as_float(s[2 * (k + i)]), __uint_as_float(s[2 * (k + i) + 1])), mul, i ? c.y : c.x), p0, p1);
+      exp2_pair<kMix, true>(k + i, fma2(pack2(__uint_as_float(s[2 * (k + i)]), __uint_as_float(s[2 * (k + i) + 1])), mul, i ? c.y : c.x), p0, p1);
       s[2 * (k + i)] = __float_as_uint(p0);
       s[2 * (k + i) + 1] = __float_as_uint(p1);
     }
