@@ -210,6 +210,16 @@ def relative_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, scal
     return _attend(q, k, v, table, max_distance, scale, _INT_MAX if window is None else window, sinks, query_start)
 
 
+def visible_softmax(scores: Tensor) -> Tensor:
+    """Softmax over the last dimension in which a score of ``-inf`` weighs nothing; a row of nothing else gives zeros."""
+    if scores.shape[-1] == 0:
+        return scores
+    top = scores.detach().amax(dim=-1, keepdim=True).clamp(min=torch.finfo(scores.dtype).min)
+    weights = torch.exp(scores - top)
+    total = weights.sum(dim=-1, keepdim=True)
+    return weights / torch.where(total == 0, torch.ones_like(total), total)
+
+
 def _expression(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor:
     wide = torch.promote_types(q.dtype, torch.float32)
     group = q.shape[2] // k.shape[2]
@@ -223,10 +233,4 @@ def _expression(q, k, v, table, max_distance, scale, window, sinks, start) -> Te
     if table is not None:
         scores = scores + table.to(wide)[:, relative_position_buckets(distance.clamp(min=0), table.shape[1], max_distance)]
     scores = scores.masked_fill(hidden, float("-inf"))
-    if k.shape[1] == 0:
-        return torch.matmul(scores, vh).transpose(1, 2).to(q.dtype)
-    top = scores.detach().amax(dim=-1, keepdim=True).clamp(min=torch.finfo(wide).min)
-    weights = torch.exp(scores - top)
-    total = weights.sum(dim=-1, keepdim=True)
-    probs = weights / torch.where(total == 0, torch.ones_like(total), total)
-    return torch.matmul(probs, vh).transpose(1, 2).to(q.dtype)
+    return torch.matmul(visible_softmax(scores), vh).transpose(1, 2).to(q.dtype)

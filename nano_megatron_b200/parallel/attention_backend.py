@@ -110,8 +110,10 @@ def flash_causal_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, dro
 def unfused_banded_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, window: Optional[int] = None, sinks: int = 0,
                              table: Optional[Tensor] = None, max_distance: int = 128, query_start: int = 0) -> Tensor:
     """Causal attention inside a window (with sinks) and / or with a relative position bias, as scores -> softmax -> @V; the
-    queries are rows from position ``query_start`` on.  ``[B, heads, S, d]``, equal numbers of heads."""
-    from ..reference.layers import banded_attn_scores, softmax_last
+    queries are rows from position ``query_start`` on.  ``[B, heads, S, d]``, equal numbers of heads.  A row whose every key the
+    table masks (``-inf``) gives zeros."""
+    from ..ops.band_attention import visible_softmax
+    from ..reference.layers import banded_attn_scores
 
     _check_qkv(q, k, v)
     if q.shape[1] != k.shape[1]:
@@ -120,7 +122,7 @@ def unfused_banded_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, w
         raise ValueError(f"query_start ({query_start}) + S_q ({q.size(2)}) exceeds S_k ({k.size(2)})")
     scores = banded_attn_scores(q, k, scale, window=window, sinks=sinks, table=table, max_distance=max_distance,
                                 query_start=query_start)
-    return torch.matmul(softmax_last(scores), v)
+    return torch.matmul(visible_softmax(scores), v)
 
 
 def flash_banded_attention(q: Tensor, k: Tensor, v: Tensor, *, scale: float, window: Optional[int] = None, sinks: int = 0,

@@ -66,7 +66,9 @@ def causal_attn_scores(q: Tensor, k: Tensor, scale: float) -> Tensor:
 def banded_attn_scores(q: Tensor, k: Tensor, scale: float, *, window: Optional[int] = None, sinks: int = 0,
                        table: Optional[Tensor] = None, max_distance: int = 128, query_start: int = 0) -> Tensor:
     """Causal scores of ``q`` rows that start at position ``query_start``: inside a window (keys of the last ``window``
-    positions and the first ``sinks`` ones) and with a bias ``table[head, bucket(distance)]`` where these are given."""
+    positions and the first ``sinks`` ones) and with a bias ``table[head, bucket(distance)]`` where these are given.  Hidden
+    keys are ``-inf``: the type's lowest value would weigh as much as an entry of the table of that value, and more than one of
+    ``-inf``.  :func:`visible_softmax` takes them."""
     from ..ops.band_attention import relative_position_buckets
 
     scores = torch.matmul(q, k.transpose(-2, -1)) * scale
@@ -77,7 +79,7 @@ def banded_attn_scores(q: Tensor, k: Tensor, scale: float, *, window: Optional[i
     hidden = distance < 0
     if window is not None:
         hidden = hidden | ((distance >= window) & (key >= sinks))
-    return scores.masked_fill(hidden, torch.finfo(scores.dtype).min)
+    return scores.masked_fill(hidden, float("-inf"))
 
 
 def softmax_last(x: Tensor) -> Tensor:
@@ -131,6 +133,7 @@ class CausalSelfAttention(nn.Module):
         return x[:, :, None].expand(b, g, n_rep, s, d).reshape(b, g * n_rep, s, d)
 
     def forward(self, x: Tensor, positions: Optional[Tensor] = None, return_activations: bool = False):
+        from ..ops.band_attention import visible_softmax
         from ..parallel.attention_backend import (
             flash_banded_attention,
             flash_causal_attention,
@@ -165,7 +168,7 @@ class CausalSelfAttention(nn.Module):
                 context = flash_banded_attention(q, k, v, scale=self.scale, dropout_p=self.config.attention_dropout, **band)
             else:
                 scores = banded_attn_scores(q, k, self.scale, **band)
-                probs = softmax_last(scores)
+                probs = visible_softmax(scores)
                 context = torch.matmul(probs, v)
         elif backend == "flash":
             context = flash_causal_attention(q, k, v, scale=self.scale, dropout_p=self.config.attention_dropout)
