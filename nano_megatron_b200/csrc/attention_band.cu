@@ -1119,15 +1119,15 @@ static int make_band_map(CUtensorMap* m, const __nv_bfloat16* ptr, const BandStr
 }
 
 // With kExact the weights go into O to twice bf16's digits: the head and what it cut off lie in the columns that the scores were
-// in, and take a product each.  D comes from O, and a bias table's gradient is a sum over dS in which D's error does not
-// cancel: with bf16 weights it was 2.2 times as far from the exact one as its own rounding at 22 keys, with both parts it is no
-// further.  Over many keys the error averages out in all buckets but the last, where the dQ kernel takes it out.  dQ and dK,
-// which also see dS rounded to bf16, were 1.5 times as far as their own rounding at 2 keys and 1.46 at 64, and are 1.42 so.  So
-// training pays for the second product where rows see few keys (8 x 512 rows, 16 heads, D = 64, window 128, bias: 20 -> 24
-// us), and nothing else does.  A variant of its own: the test inside the loop cost the others 10 percent through registers.
+// in, and take a product each.  D comes from O, and a bias table's gradient is a sum over dS in which D's error does not cancel,
+// but adds up where a bucket has much of the rows' weight, be it the last one or a wide or favoured one before it: with bf16
+// weights it was 2.2 times as far from the exact one as its own rounding at 22 keys, up to 14 times over thousands (2 to 64
+// buckets), 7.5 times with a table that favours one bucket; with both parts it is no further.  The second product is
+// paid by every training step with a table (8192 x 16 heads, D = 128: 1258 -> 1348 us; 2 x 2048, D = 64: 160 -> 168 us).
 static bool exact_weights(const BandArgs& a) {
+  if (a.m == nullptr) return false;
   const long long keys = std::min<long long>(a.Skv, static_cast<long long>(a.window) + a.sinks);
-  return a.rest_rows > 0 && keys <= (a.table != nullptr ? 512 : 64);
+  return a.table != nullptr || keys <= 64;
 }
 template <int D>
 static cudaError_t launch_band_fwd(const BandFwdParams& p, cudaStream_t s) {
@@ -1289,11 +1289,6 @@ struct BandGroups {
 // up where terms of dS cancel (few keys: 4.7e-3 of dQ's norm instead of 2.3e-3), and, summed over thousands of keys, is as large
 // as the gradient of the last bucket (1.6e-2 of it).  So a forward pass that will be differentiated also keeps what the rounding
 // cut off, as another bf16 value: of all rows with a bias, else of those that see few keys (the caller says up to which row).
-//
-// What is still missing from O is the rounding of the forward pass's weights.  A row's dS sum to nothing, those computed here to
-// the error of its D: times the weights of the last bucket it is taken out of that bucket's gradient, where terms cancel most
-// (the others have few keys a row).  Without, the table's gradient was up to 14 times as far from the exact one as its own
-// rounding (2 to 64 buckets, 100 to 4000 rows).
 //
 // dtable: inside tiles that meet distances below t_last the sums along the diagonals (equal distance) are formed by passing a
 // running sum from lane to lane, one row down per column; they are then added by bucket.  All other tiles belong to the last
@@ -1557,7 +1552,7 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[qs]);
       }
-      float ds_far = 0.f, ds_all = 0.f, p_far = 0.f;  // sums over the last bucket's dS in tiles that are all its own, all dS, its weights
+      float ds_far = 0.f;  // sum of dS in tiles that are all the last bucket's own
       for (int u = 0; u < n; ++u, ++step) {
         const int kv0 = tile_at(w.t, u) * 128, k0 = kv0 + quarter * 32;
         NMB_BAND_WAIT(&sdp_full[g], step & 1, 90);
@@ -1610,27 +1605,13 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         if (lane == 0) mbar_arrive(&ds_full[2 * g + (step & 1)]);
         if (want_table) {
           if (!near) {
-            uint64_t sum = pack2(0.f, 0.f), sum_p = pack2(p_far, 0.f);
+            uint64_t sum = pack2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              sum = add2(sum, pack2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])));
-              sum_p = add2(sum_p, pack2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])));
-            }
-            float s0, s1, p0, p1;
+            for (int k = 0; k < 32; k += 2) sum = add2(sum, pack2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])));
+            float s0, s1;
             unpack2(sum, s0, s1);
-            unpack2(sum_p, p0, p1);
             ds_far += s0 + s1;
-            ds_all += s0 + s1;
-            p_far = p0 + p1;
           } else {
-            const uint32_t far = low_bits(pos - p.t_last - k0 + 1);  // keys of the last bucket
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              sum += __uint_as_float(dp[k]);
-              if ((far >> k) & 1u) p_far += __uint_as_float(s[k]);
-            }
-            ds_all += sum;
             // diagonal e holds distance base + e; lane 31 completes one of them per column, the others stay behind at the end
             const int base = pmin + quad * 32 - k0 - 31;
             float run = 0.f;
@@ -1712,10 +1693,6 @@ __global__ void __launch_bounds__(kBandThreads, 1) band_bwd_dq_kernel(const __gr
         if (lane == 0) mbar_arrive(dq_empty);
       }
       if (want_table) {
-        diag[lane] = ds_all;
-        together();
-        const float* row_of = bins + kComputeWarps * kMaxBuckets + quad * 64 + lane;  // the row's four threads
-        ds_far -= ((row_of[0] + row_of[4 * 64]) + (row_of[8 * 64] + row_of[12 * 64])) * p_far;
         const float last = warp_sum(ds_far);
         if (lane == 0) my_bins[a.buckets - 1] += last;
         together();

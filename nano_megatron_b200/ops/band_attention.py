@@ -18,11 +18,14 @@ a data-parallel wrapper), else through autograd.
 bf16 CUDA tensors with a head_dim of 64, 96 or 128 go to the kernels; everything else (CPU, fp32, other
 head sizes) to the plain expression at the end of this file, in fp32 or wider.  The kernels multiply whole
 tiles of 128 keys, with zero weights where a key is masked: as in the plain expression, keys and values have
-to be finite in masked places too.  Values that are not finite show: a row that sees a score of NaN or +inf (an overflow of
-fp32 among them, or an entry of the table) is NaN, and so are the gradients that it takes part in; a score of -inf is a weight
-of 0, as an entry of -inf in the table is, and a row that has nothing else gives zeros.  Where rows see few keys, a call that will be differentiated carries the
-weights to twice bf16's digits, for the gradients' sake: its output may differ from that of the same call without
-gradients by the roundings of the weights.  Results do not depend on timing: the same call gives the same bits.
+to be finite in masked places too.  Values that are not finite show: a row that sees a score of NaN or +inf
+(an overflow of fp32 among them, or an entry of the table) is NaN, and so are the gradients that it takes part
+in; a score of -inf is a weight of 0, as an entry of -inf in the table is, and a row that has nothing else
+gives zeros.
+
+With a bias table, or where rows see few keys, a call that will be differentiated carries the weights to twice
+bf16's digits, for the gradients' sake: its output may differ from that of the same call without gradients by
+the roundings of the weights.  Results do not depend on timing: the same call gives the same bits.
 """
 from __future__ import annotations
 
