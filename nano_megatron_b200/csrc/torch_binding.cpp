@@ -123,11 +123,16 @@ struct BandAttention : torch::autograd::Function<BandAttention> {
     Tensor rest, stats;
     if (train) {
       // Rows that see kFewKeys or more do without: there the error of D is below a tenth of the other roundings' (it falls with
-      // the root of their number).  The last bucket's gradient is a sum over all rows, and wants them all.
+      // the root of their number).  A table's gradient is a sum over all rows, and wants them all.  Later rows see more keys until
+      // the window or the keys end, then fewer: those that see few are the first ones and, where the keys end, the last ones.
       constexpr int64_t kFewKeys = 256;
-      const int64_t rows = q.size(1);
-      const int64_t kept = table.defined() || std::min<int64_t>(window, kFewKeys) + std::min<int64_t>(sinks, kFewKeys) <= kFewKeys
-                               ? rows : std::min(rows, std::max<int64_t>(0, kFewKeys - start));
+      const int64_t rows = q.size(1), keys = k.size(1);
+      auto few = [&](int64_t position) {
+        const int64_t first = std::max<int64_t>(0, position - window + 1);
+        const int64_t band = std::max<int64_t>(0, std::min(position, keys - 1) - first + 1);
+        return band + std::min(sinks, std::min(first, keys)) < kFewKeys;
+      };
+      const int64_t kept = table.defined() || few(start + rows - 1) ? rows : std::min(rows, std::max<int64_t>(0, kFewKeys - start));
       rest = at::empty({q.size(0), kept, q.size(2), q.size(3)}, q.options());
       stats = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
     }
