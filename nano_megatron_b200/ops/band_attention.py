@@ -139,6 +139,17 @@ def _check_buckets(num_buckets: int, max_distance: int) -> None:
                          f"got {max_distance}")
 
 
+def check_band(window: Optional[int], sinks: int, num_buckets: Optional[int], max_distance: Optional[int]) -> None:
+    """Refuses what the operators refuse of these (``None`` for a window or a table that is not there)."""
+    if window is not None:
+        _check_int("window", window, 1)
+    _check_int("sinks", sinks, 0)
+    if num_buckets is not None:
+        _check_int("the number of buckets", num_buckets, 2)
+        _check_int("max_distance", max_distance, 1)
+        _check_buckets(num_buckets, max_distance)
+
+
 @functools.lru_cache(maxsize=4096)
 def _check_shapes(q, k, v, floating, buckets, max_distance, scale, start) -> None:
     if len(q) != 4 or len(k) != 4 or len(v) != 4:

@@ -58,14 +58,13 @@ class ReferenceGPTConfig:
             self.rotary_dim = head_dim
         if self.num_query_groups is None:
             self.num_query_groups = self.num_heads
-        if self.attention_window is not None and self.attention_window < 1:
-            raise ValueError(f"attention_window must be at least 1, got {self.attention_window}")
-        if self.attention_sinks < 0 or (self.attention_sinks > 0 and self.attention_window is None):
-            raise ValueError(f"attention_sinks ({self.attention_sinks}) must not be negative and need an attention_window")
-        if self.position_embedding_type == "relative" and not \
-                2 <= self.relative_buckets < 2 * self.relative_max_distance + 2:
-            raise ValueError(f"relative_max_distance ({self.relative_max_distance}) must be above half of relative_buckets "
-                             f"({self.relative_buckets}), of which there must be two at least")
+        from ..ops.band_attention import check_band
+
+        relative = self.position_embedding_type == "relative"
+        check_band(self.attention_window, self.attention_sinks, self.relative_buckets if relative else None,
+                   self.relative_max_distance if relative else None)
+        if self.attention_sinks > 0 and self.attention_window is None:
+            raise ValueError(f"attention_sinks ({self.attention_sinks}) need an attention_window")
         # Modules are always built in fp32; callers cast afterwards (as the
         # reference's benchmarks do with ``model.to(torch.bfloat16)``).
         self.dtype = torch.float32

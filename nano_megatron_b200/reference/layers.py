@@ -69,8 +69,9 @@ def banded_attn_scores(q: Tensor, k: Tensor, scale: float, *, window: Optional[i
     positions and the first ``sinks`` ones) and with a bias ``table[head, bucket(distance)]`` where these are given.  Hidden
     keys are ``-inf``: the type's lowest value would weigh as much as an entry of the table of that value, and more than one of
     ``-inf``.  :func:`visible_softmax` takes them."""
-    from ..ops.band_attention import relative_position_buckets
+    from ..ops.band_attention import check_band, relative_position_buckets
 
+    check_band(window, sinks, None if table is None else table.shape[1], max_distance)
     scores = torch.matmul(q, k.transpose(-2, -1)) * scale
     key = torch.arange(k.size(-2), device=q.device)
     distance = torch.arange(query_start, query_start + q.size(-2), device=q.device)[:, None] - key
