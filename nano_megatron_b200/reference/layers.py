@@ -110,7 +110,8 @@ class CausalSelfAttention(nn.Module):
             self.k_proj = nn.Linear(config.hidden_size, kv_dim, bias=qkv_bias)
             self.v_proj = nn.Linear(config.hidden_size, kv_dim, bias=qkv_bias)
         self.out_proj = nn.Linear(config.hidden_size, config.hidden_size, bias=config.use_bias)
-        self.banded = config.attention_window is not None or config.position_embedding_type == "relative"
+        # (a configuration of the reference project has no window)
+        self.banded = getattr(config, "attention_window", None) is not None or config.position_embedding_type == "relative"
         self.rel_bias: Optional[nn.Parameter] = None
         if config.position_embedding_type == "relative":
             self.rel_bias = nn.Parameter(torch.zeros(config.num_heads, config.relative_buckets))

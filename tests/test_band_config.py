@@ -1,11 +1,17 @@
 """What a configuration accepts of windows and relative positions is what the operators accept."""
 from __future__ import annotations
 
+from dataclasses import asdict
+from types import SimpleNamespace
+
 import pytest
 import torch
 
+from nano_megatron_b200.models import build_tp_gpt_from_reference
 from nano_megatron_b200.parallel import unfused_banded_attention
 from nano_megatron_b200.reference import ReferenceGPT, ReferenceGPTConfig
+
+from ._thread_ranks import run_ranks, thread_context
 
 
 def _config(**knobs):
@@ -43,3 +49,17 @@ def test_the_unfused_entry_point_refuses_the_same(kw, error):
     q = torch.zeros(1, 2, 4, 8)
     with pytest.raises(error):
         unfused_banded_attention(q, q, q, scale=1.0, **kw)
+
+
+def test_a_configuration_without_these_fields():
+    """The reference project's own object, which knows neither windows nor relative positions."""
+    fields = {n: v for n, v in asdict(_config()).items() if not n.startswith(("attention_window", "attention_sinks", "relative_"))}
+    torch.manual_seed(0)
+    ref = ReferenceGPT(SimpleNamespace(**fields))
+    ids = torch.randint(0, 32, (1, 8))
+
+    def rank_fn(rank, be, model):
+        return model(ids)
+
+    got = run_ranks(1, rank_fn, lambda rank, be: build_tp_gpt_from_reference(ref, thread_context(rank, be, tp=1)))[0]
+    torch.testing.assert_close(got, ref(ids), rtol=1e-5, atol=1e-5)
