@@ -11,7 +11,6 @@
 #include <torch/library.h>
 
 #include <array>
-#include <cmath>
 #include <map>
 #include <mutex>
 #include <vector>
@@ -223,7 +222,8 @@ bool ready(const Tensor& q, const Tensor& k, const Tensor& v, const std::optiona
   const int64_t d = q.size(3);
   if (k.sizes() != v.sizes() || q.size(0) != k.size(0) || d != k.size(3) || (d != 64 && d != 96 && d != 128) || q.size(2) % k.size(2) != 0)
     return false;
-  if (!(std::isfinite(scale) && scale > 0.0) || window < 1 || window > kIntMax || sinks < 0 || sinks > kIntMax || start < 0 ||
+  constexpr double kScaleLimit = 0x1p126;  // held in fp32, times log2(e)
+  if (!(scale >= 1.0 / kScaleLimit && scale <= kScaleLimit) || window < 1 || window > kIntMax || sinks < 0 || sinks > kIntMax || start < 0 ||
       start > kMaxPosition || start + q.size(1) > kMaxPosition || k.size(1) > kMaxPosition || g_status[q.device().index()] == nullptr)
     return false;
   if (!table.has_value()) return true;

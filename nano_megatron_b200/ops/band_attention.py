@@ -43,6 +43,7 @@ MAX_BUCKETS = 128        # sizes of the kernels' tables
 MAX_DISTANCE = 2048
 _MAX_POSITION = 2 ** 30
 _INT_MAX = 2 ** 31 - 1
+_SCALE_LIMIT = 2.0 ** 126  # held in fp32 by the kernels, times log2(e)
 
 
 @functools.lru_cache(maxsize=None)
@@ -162,8 +163,8 @@ def _check_shapes(q, k, v, floating, buckets, max_distance, scale, start) -> Non
         raise ValueError(f"query heads must be a multiple of key heads; got q={tuple(q)}, k={tuple(k)}")
     if not floating:
         raise ValueError("q, k, v must be floating-point tensors")
-    if not (math.isfinite(scale) and scale > 0.0):
-        raise ValueError(f"scale must be finite and positive, got {scale}")
+    if not 1.0 / _SCALE_LIMIT <= scale <= _SCALE_LIMIT:  # a NaN neither
+        raise ValueError(f"scale must be positive and within 2 ** -126 and 2 ** 126, got {scale}")
     if start + q[1] > _MAX_POSITION or k[1] > _MAX_POSITION:
         raise ValueError(f"positions must stay below {_MAX_POSITION}; got query_start {start}, q={tuple(q)}, k={tuple(k)}")
     if buckets is not None:
