@@ -2255,7 +2255,7 @@ __global__ void __launch_bounds__(256) band_finish_kernel(const __grid_constant_
 // 0.4 percent behind the best one of all SMs' loads, never cutting 58 percent.
 static void plan_pieces(BandBwdParams& p) {
   const BandArgs& a = p.a;
-  const int sms = sm_count(), n_hb = a.Hkv * a.B, piece_cost = 2 + a.d / 32;
+  const int sms = std::max(1, sm_count()), n_hb = a.Hkv * a.B, piece_cost = 2 + a.d / 32;
   constexpr int kMaxRounds = 16;  // looked at one by one; cutting gains nothing where there are more
   int longest = 1, longest_sink = 1;
   for (int t = 0; t < p.n_kt; ++t) {
@@ -2382,6 +2382,19 @@ static int band_check(const BandArgs* a) {
   return 0;
 }
 
+static int fwd_check(const BandArgs* a) {
+  if (int bad = band_check(a)) return bad;
+  if (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->o == nullptr || (a->m == nullptr) != (a->l == nullptr)) return kBadArgument;
+  if (a->rest_rows < 0 || a->rest_rows > a->Sq || (a->rest_rows > 0 && a->o_rest == nullptr)) return kBadArgument;
+  return 0;
+}
+static int bwd_check(const BandArgs* a) {
+  if (int bad = fwd_check(a)) return bad;
+  if (a->m == nullptr || a->dout == nullptr || a->dq == nullptr || a->dk == nullptr || a->dv == nullptr || a->scratch == nullptr) return kBadArgument;
+  if (a->dtable != nullptr && a->table == nullptr) return kBadArgument;
+  return 0;
+}
+
 extern "C" int nmb_band_args_size() { return static_cast<int>(sizeof(BandArgs)); }
 
 extern "C" long long nmb_band_bwd_scratch(const BandArgs* a) {
@@ -2429,7 +2442,7 @@ extern "C" long long nmb_band_fwd_scratch(const BandArgs* a) {
 extern "C" int nmb_band_fwd(const BandArgs* a, void* stream) { return nmb_band_fwd_split(a, nullptr, stream); }
 
 extern "C" int nmb_band_fwd_split(const BandArgs* a, float* scratch, void* stream) {
-  if (int bad = band_check(a)) return bad;
+  if (int bad = fwd_check(a)) return bad;
   if (reinterpret_cast<uintptr_t>(scratch) % 32 != 0) return kBadArgument;
   (void)cudaGetLastError();
   BandFwdParams p;
@@ -2478,13 +2491,14 @@ extern "C" int nmb_band_bwd_plan(const BandArgs* a, BandPlan* plan) {
 }
 
 extern "C" int nmb_band_bwd(const BandArgs* a, void* stream) {
+  if (int bad = bwd_check(a)) return bad;
   BandPlan plan;
   if (int bad = nmb_band_bwd_plan(a, &plan)) return bad;
   return nmb_band_bwd_planned(a, &plan, stream);
 }
 
 extern "C" int nmb_band_bwd_planned(const BandArgs* a, const BandPlan* plan, void* stream) {
-  if (int bad = band_check(a)) return bad;
+  if (int bad = bwd_check(a)) return bad;
   (void)cudaGetLastError();
   BandBwdParams p;
   const BandScratch w = plan_bwd(p, *a, plan);

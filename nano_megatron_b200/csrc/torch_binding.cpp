@@ -5,6 +5,7 @@
 // on the GPU for 8 x 512 tokens.  Everything that a call does between the check of its arguments and the launch is here.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -234,9 +235,26 @@ bool ready(const Tensor& q, const Tensor& k, const Tensor& v, const std::optiona
   return g_limits.count({table->size(1), max_distance}) != 0;  // what is there has passed the checks
 }
 
+// Tensors without memory (fake ones, of a trace) and calls under a mode that records operators: the kernels would run on null
+// addresses, or beside the record.
+void refuse_tracing(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t.unsafeGetTensorImpl()->is_python_dispatch(),
+                              "banded attention: the kernels cannot be traced; wrap the call in torch.compiler.disable");
+}
+void refuse_tracing() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  TORCH_CHECK_NOT_IMPLEMENTED(!Modes::get_mode(Key::FAKE).has_value() && !Modes::get_mode(Key::PROXY).has_value() &&
+                                  !Modes::get_mode(Key::FUNCTIONAL).has_value(),
+                              "banded attention: the kernels cannot be traced; wrap the call in torch.compiler.disable");
+}
+
 // None where the call is not one for the kernels, or not yet.
 std::optional<Tensor> band_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& table, double scale,
                                      int64_t window, int64_t sinks, int64_t start, int64_t max_distance) {
+  refuse_tracing();
+  for (const Tensor* t : {&q, &k, &v}) refuse_tracing(*t);
+  if (table.has_value()) refuse_tracing(*table);
   if (!ready(q, k, v, table, scale, window, sinks, start, max_distance)) return std::nullopt;
   const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                     (table.has_value() && table->requires_grad()));

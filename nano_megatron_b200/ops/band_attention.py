@@ -26,6 +26,9 @@ gives zeros.
 With a bias table, or where rows see few keys, a call that will be differentiated carries the weights to twice
 bf16's digits, for the gradients' sake: its output may differ from that of the same call without gradients by
 the roundings of the weights.  Results do not depend on timing: the same call gives the same bits.
+
+The kernels cannot be traced (``torch.compile``, fake tensors) nor transformed (``torch.func``): such calls are
+refused.
 """
 from __future__ import annotations
 
@@ -171,6 +174,14 @@ def _check_shapes(q, k, v, floating, buckets, max_distance, scale, start) -> Non
         _check_buckets(buckets, max_distance)
 
 
+def _refuse_tracing(*tensors) -> None:
+    """What ``csrc/torch_binding.cpp`` refuses, before a device is set up under a mode that hands out tensors without memory."""
+    keys = torch._C._TorchDispatchModeKey
+    if (any(torch._C._get_dispatch_mode(key) is not None for key in (keys.FAKE, keys.PROXY, keys.FUNCTIONAL))
+            or any(t is not None and torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python) for t in tensors)):
+        raise NotImplementedError("banded attention: the kernels cannot be traced; wrap the call in torch.compiler.disable")
+
+
 def _attend(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor:
     if _ready and q.is_cuda and type(scale) is float and type(window) is type(sinks) is type(start) is type(max_distance) is int:
         # one look from C++ in place of those below, which took as long as the rest of a call together
@@ -195,6 +206,7 @@ def _attend(q, k, v, table, max_distance, scale, window, sinks, start) -> Tensor
         _check_int("max_distance", max_distance, 1)
     _check_shapes(q.shape, k.shape, v.shape, q.is_floating_point(), buckets, max_distance, scale, start)
     if band_attention_supported(q) and q.numel() and k.numel():
+        _refuse_tracing(q, k, v, table)
         if table is not None:
             if table.dtype not in (torch.bfloat16, torch.float32):
                 raise ValueError(f"table must be bfloat16 or float32, got {table.dtype}")
