@@ -51,7 +51,8 @@ bool strides_fit(const Tensor& t) {
   return true;
 }
 Tensor readable(const Tensor& t) {
-  if (!strides_fit(t) || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0) return t.clone(at::MemoryFormat::Contiguous);
+  if (!strides_fit(t)) return t.clone(at::MemoryFormat::Contiguous);
+  if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0) return at::empty_strided(t.sizes(), t.strides(), t.options()).copy_(t);
   return t;
 }
 // A gradient buffer: laid out as the input where that is dense, so that it can become the leaf's gradient as it is.
