@@ -480,7 +480,6 @@ struct BandFwdParams {
   BandArgs a;
   int pair;     // 0: one tile an item, 1: two neighbouring tiles, 2: two heads
   int n_qt;     // query tiles of a head
-  int s_pad;    // rows of the statistics: n_qt * 128
   int n_items;
   int t_last;   // first distance of the last bucket
   int pieces;   // parts of a tile's keys, with pair == 0 only: sums and statistics of each go to `part`
@@ -1144,9 +1143,10 @@ template <int D>
 static cudaError_t launch_band_join(const BandFwdParams& p, cudaStream_t s) {
   return launch_pdl(band_join_kernel<D>, dim3(static_cast<unsigned>(p.n_items / p.pieces * 16)), dim3(256), 0, s, p);
 }
-// Into how many pieces the keys of a query tile are cut where there are not half as many tiles as SMs, four key tiles to a piece
-// at least: one row over 8192 keys, 16 heads of 128: 115 -> 25 us; over 1024 keys 18 -> 15 us.  (As a variant of its own: the
-// pieces cost the others 2 to 5 percent.)
+// Into how many pieces the keys of a query tile are cut where there are not half as many tiles as SMs, three or four key tiles to
+// a piece at least: one row over 8192 keys, 16 heads of 128 (16/4 heads alike): 115 -> 25 us; over 1024 keys 18 -> 15 us.  The
+// window's tiles alone are counted and cut, sinks stay with the first piece: one row with a window of 64 and 4096 sinks, 61 us.
+// (As a variant of its own: the pieces cost the others 2 to 5 percent.)
 constexpr int kSplitKeyTiles = 8;
 static int fwd_pieces(const BandArgs& a) {
   const long long tiles = static_cast<long long>((a.Sq + 127) / 128) * a.Hq * a.B;
@@ -2456,10 +2456,12 @@ extern "C" int nmb_band_fwd_split(const BandArgs* a, float* scratch, void* strea
     if (make_band_map(&p.rest_map, a->o_rest, BandStride{a->rest_rows * row, row, a->d}, a->d, a->rest_rows, a->Hq, a->B)) return 106;
   }
   p.n_qt = (a->Sq + 127) / 128;
-  p.s_pad = p.n_qt * 128;
   p.t_last = a->table == nullptr ? 0 : a->limit[a->buckets - 2];
   const long long tiles = static_cast<long long>(p.n_qt) * a->Hq * a->B;
-  // one tile an item while every tile can have an SM of its own
+  // One tile an item while every tile can have an SM of its own.  From there on pairs: with a window of 256 over 192 tiles 11.0 us
+  // where single tiles take 12.9 (D = 64), over 256 tiles 13.6 and 17.6 (D = 96).  Causal rows over 8 to 16 key tiles would be
+  // better off as single tiles up to about 300 (192 tiles 19.0 and 15.8 us, 256 tiles 32.9 and 27.9, 320 tiles 33.3 and 36.3): the
+  // pairs are one round of long items there.
   p.pair = tiles <= sm_count() ? 0 : (a->Hq / a->Hkv) % 2 == 0 ? 2 : 1;
   p.pieces = scratch == nullptr ? 1 : fwd_pieces(*a);
   p.part = scratch;

@@ -198,9 +198,11 @@ class TPCausalSelfAttention(nn.Module):
         return OF.rope_bshd(q, pos, self._inv_freq_dev), OF.rope_bshd(k, pos, self._inv_freq_dev)
 
     def _forward_banded(self, x: Tensor, positions: Optional[Tensor], residual: Optional[Tensor]) -> Tensor:
-        """bf16 GPU path of attention inside a window and / or with a relative position bias.  The kernels read the slices of
-        the packed projection in place and write the gradients of all three into one buffer.  Under context parallelism the
-        keys and values of all ranks are gathered; a rank's queries are a shard of the sequence to the kernels."""
+        """bf16 GPU path of attention inside a window and / or with a relative position bias.  Without rotary positions the
+        kernels read the slices of the packed projection in place and write the gradients of all three into one buffer; with
+        them q and k are rotated copies (a copy and a kernel each, forward and backward), and the gradients of the packed
+        projection are joined by another.  Under context parallelism the keys and values of all ranks are gathered; a rank's
+        queries are a shard of the sequence to the kernels."""
         from ..ops.attention import split_packed_qkv
         from ..ops.band_attention import relative_bias_attention, window_attention
 
