@@ -252,9 +252,12 @@ void refuse_tracing() {
 // None where the call is not one for the kernels, or not yet.
 std::optional<Tensor> band_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& table, double scale,
                                      int64_t window, int64_t sinks, int64_t start, int64_t max_distance) {
-  refuse_tracing();
-  for (const Tensor* t : {&q, &k, &v}) refuse_tracing(*t);
-  if (table.has_value()) refuse_tracing(*table);
+  const int64_t d = q.defined() && q.dim() == 4 ? q.size(3) : 0;
+  if (q.defined() && q.scalar_type() == at::kBFloat16 && (d == 64 || d == 96 || d == 128)) {  // others take the plain expression
+    refuse_tracing();
+    for (const Tensor* t : {&q, &k, &v}) refuse_tracing(*t);
+    if (table.has_value()) refuse_tracing(*table);
+  }
   if (!ready(q, k, v, table, scale, window, sinks, start, max_distance)) return std::nullopt;
   const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                     (table.has_value() && table->requires_grad()));

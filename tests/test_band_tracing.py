@@ -87,5 +87,7 @@ def test_traces_are_refused_after_an_ordinary_call():
             fake = _fake(grad)
             with pytest.raises(NotImplementedError, match="traced"):
                 relative_bias_attention(fake, fake, fake, table, 0.125)
+        wide = torch.empty(2, 40, 2, 64, device="cuda")  # not for the kernels: the expression
+        assert window_attention(wide, wide, wide, 0.125, window=9).shape == wide.shape
     apart = torch.compiler.disable(window_attention)
     assert torch.equal(torch.compile(lambda t: apart(t, t, t, 0.125, window=9) * 2, backend="eager")(q), want * 2)
